@@ -5,6 +5,8 @@ and the clipped policy and paired preference losses over rows of logits (edgehip
 `run` with own = False is each operator in elementary torch operations, in 32 bits; with own = True it is the calls a
 user makes of this package.  `exact` is the definition in 64 bits, written apart from both."""
 import math
+import os
+import sys
 
 import torch
 
@@ -192,6 +194,11 @@ def prepare(case, seed):
 
 
 # ---- the framework's calls ---------------------------------------------------------------------------------------
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'graph-generation-edge_amd')
+if PACKAGE not in sys.path:
+    sys.path.append(PACKAGE)                                       # imported by the calls below only
+
+
 def _own_norm(s):
     import edgehip.block as block
     kw = {k: s[k] for k in ('w_pre', 'b_pre', 'w_post', 'b_post', 'gate', 'row_ptr', 'res_scale')}
@@ -297,7 +304,7 @@ def _plain_pack(x):
     m, k = x.shape
     x = torch.nn.functional.pad(x.float(), (0, -k % GROUP)).view(m, -1, GROUP)
     f, e = torch.frexp(x.abs().amax(2, keepdim=True))
-    e = torch.where(f <= 127 / 128, e - 7, e - 6).clamp(-120, 121)
+    e = torch.where(f <= 127 / 128, e - 7, e - 6).clamp_min(-120)
     up, down = (((127 + v) << 23).view(torch.float32) for v in (e, -e))           # 2^e and 2^-e to the bit
     return (torch.round(x * down) * up).view(m, -1)[:, :k]
 
@@ -449,7 +456,7 @@ def _pack64(x):
     out[:, :k] = x.double()
     out = out.view(m, -1, GROUP)
     top = out.abs().amax(2, keepdim=True)
-    steps = torch.tensor([math.ldexp(1.0, i) for i in range(-120, 122)], dtype=torch.float64, device=DEV)
+    steps = torch.tensor([math.ldexp(1.0, i) for i in range(-120, 123)], dtype=torch.float64, device=DEV)
     step = steps[torch.searchsorted(127 * steps, top.contiguous())]              # the smallest with top <= 127 steps
     return (torch.round(out / step) * step).view(m, -1)[:, :k]
 
