@@ -10,3 +10,7 @@ from . import shard  # noqa: F401
 from .trainer import make_optimizer, train_step  # noqa: F401
 from . import stats  # noqa: F401
 from .stats import NetworkEvaluator, edge_overlap, graph_statistics  # noqa: F401
+from . import block, ckpt8, tune  # noqa: F401
+from .block import gate_norm  # noqa: F401
+from .ckpt8 import act8, linear8, pack8  # noqa: F401
+from .tune import policy_loss, policy_loss_grad, preference_loss, preference_loss_grad, row_logp  # noqa: F401

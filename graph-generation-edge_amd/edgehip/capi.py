@@ -61,6 +61,29 @@ class GnnParams(C.Structure):
                            'final_w0', 'final_b0', 'final_w2', 'final_b2', 'final_w4', 'final_b4', 'pos_emb')]
 
 
+class GateNorm(C.Structure):
+    _fields_ = [('rows', C.c_int64)] + \
+        [(n, C.c_int32) for n in ('dim', 'stream_dtype', 'branch_dtype', 'kind', 'pre', 'post', 'param_dtype', 'gate_kind',
+                                  'gate_dtype', 'groups')] + \
+        [(n, vp) for n in ('w_pre', 'b_pre', 'w_post', 'b_post', 'gate', 'row_ptr')] + \
+        [('res_scale', C.c_float), ('eps', C.c_float)]
+
+
+class LogitRows(C.Structure):
+    _fields_ = [('rows', C.c_int64), ('row_stride', C.c_int64), ('classes', C.c_int32), ('dtype', C.c_int32),
+                ('num_seqs', C.c_int32), ('reserved', C.c_int32), ('logits', vp), ('taken', vp), ('mask', vp), ('seq_ptr', vp)]
+
+
+class Policy(C.Structure):
+    _fields_ = [('old_logp', vp), ('advantage', vp), ('ref_logp', vp), ('weight', vp), ('clip_lo', C.c_double),
+                ('clip_hi', C.c_double), ('kl_coef', C.c_double), ('advantage_per_row', C.c_int32), ('mean', C.c_int32)]
+
+
+class Preference(C.Structure):
+    _fields_ = [('ref_logp', vp), ('weight', vp), ('beta', C.c_double), ('label_smoothing', C.c_double), ('kind', C.c_int32),
+                ('mean', C.c_int32)]
+
+
 EXPORTS = {
     'edgehip_degree_from_adj': [C.POINTER(Layout), vp, vp, vp],
     'edgehip_active_select_sample': [C.POINTER(Layout), vp, vp, vp, vp, C.c_int32, vp, C.POINTER(Rng), vp, vp, vp, vp, vp],
@@ -123,8 +146,25 @@ EXPORTS = {
                                   C.c_int64, C.c_int64, vp, vp, vp, C.POINTER(Dropout), vp, C.c_size_t, vp],
     'edgehip_train_backward_cap': [C.POINTER(Layout), C.POINTER(GnnParams), C.POINTER(GnnParams), vp, vp, vp, vp, vp, vp,
                                    C.c_int64, C.c_int64, vp, vp, vp, vp, C.c_size_t, vp],
+    # norms around a gated residual step, 8-bit checkpoints, tuning losses (csrc/block.hip, ckpt8.hip, tune.hip)
+    'edgehip_gate_norm_fwd': [C.POINTER(GateNorm), vp, vp, vp, vp, vp, vp],
+    'edgehip_gate_norm_bwd': [C.POINTER(GateNorm), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp],
+    'edgehip_pack8': [C.c_int32, vp, C.c_int64, C.c_int64, vp, vp, vp],
+    'edgehip_unpack8': [C.c_int32, vp, vp, C.c_int64, C.c_int64, vp, vp],
+    'edgehip_act8_fwd': [C.c_int32, C.c_int32, vp, C.c_int64, C.c_int64, vp, vp, vp, vp],
+    'edgehip_act8_bwd': [C.c_int32, C.c_int32, vp, vp, vp, C.c_int64, C.c_int64, vp, vp],
+    'edgehip_linear8_bwd_weight': [C.c_int32, vp, vp, vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp, C.c_size_t, vp],
+    'edgehip_row_logp': [C.POINTER(LogitRows), vp, vp],
+    'edgehip_policy_loss_fwd': [C.POINTER(LogitRows), C.POINTER(Policy), vp, vp, vp, vp, vp, C.c_size_t, vp],
+    'edgehip_policy_loss_bwd': [C.POINTER(LogitRows), C.POINTER(Policy), vp, vp, C.c_size_t, vp],
+    'edgehip_policy_loss_grad': [C.POINTER(LogitRows), C.POINTER(Policy), vp, vp, vp, vp, vp, vp, C.c_size_t, vp],
+    'edgehip_preference_loss_fwd': [C.POINTER(LogitRows), C.POINTER(Preference), vp, vp, vp, C.c_size_t, vp],
+    'edgehip_preference_loss_bwd': [C.POINTER(LogitRows), C.POINTER(Preference), vp, vp, C.c_size_t, vp],
 }
 SIZE_EXPORTS = {
+    'edgehip_gate_norm_workspace_bytes': [C.POINTER(GateNorm)],
+    'edgehip_linear8_workspace_bytes': [C.c_int32, C.c_int64, C.c_int32, C.c_int32],
+    'edgehip_tune_workspace_bytes': [C.POINTER(LogitRows)],
     'edgehip_gnn_folded_floats': [C.POINTER(GnnParams)],
     'edgehip_gnn_workspace_bytes': [C.POINTER(Layout), C.POINTER(GnnParams)],
     'edgehip_train_workspace_bytes': [C.POINTER(Layout), C.POINTER(GnnParams), C.c_int64],
@@ -208,6 +248,34 @@ def stream_ptr():
     if torch.cuda.is_available():
         return torch.cuda.current_stream().cuda_stream
     return None
+
+
+# ---- argument checks shared by the operators over several types (block, ckpt8, tune) ----------------------
+F32, BF16, F16 = 0, 1, 2
+
+
+def dtype_code(what, name, t):
+    import torch
+    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f'{what}: {name} must be fp32, bf16 or fp16, got {t.dtype}')
+    return code
+
+
+def same_device(what, name, t, dev):
+    if t.device != dev:
+        raise ValueError(f'{what}: {name} is on {t.device}, the other tensors on {dev}')
+
+
+def on_gpu(what, t):
+    if not t.is_cuda:
+        raise ValueError(f'{what}: the tensors must be on a GPU (there is no CPU path), got {t.device}')
+
+
+def device_of(t):
+    """with device_of(t): the tensor's GPU is current, so that `stream_ptr` names a stream of it."""
+    import torch
+    return torch.cuda.device(t.device)
 
 
 # One pool of side streams per device for everything in this package (the sampler's sub-batch streams, the training

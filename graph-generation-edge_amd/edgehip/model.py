@@ -720,7 +720,8 @@ class BinomialDiffusionActive(nn.Module):
             if differentiable:
                 net.weights_changed()       # an optimizer step may follow this loss (see weights_changed)
             counts = None
-            if getattr(self, 'train_form', 'fused') != 'ops':
+            form = getattr(self, 'train_form', 'fused')           # 'fused', 'ops', 'ops8' (ops with 8-bit checkpoints)
+            if form not in ('ops', 'ops8'):
                 # the node part of the network needs no active pairs: it is queued before the step's only host sync
                 # (the pair counts), read back on a side stream behind the offsets kernel
                 after = torch.cuda.Event()
@@ -730,8 +731,8 @@ class BinomialDiffusionActive(nn.Module):
             self.materialize_actives(batch, counts)
             row, col = batch.active_row, batch.active_col
             tgt, pair_graph = train.pair_targets(batch, adj_tm1, row, col)
-            fwd = train.tgnn_ce_forward if getattr(self, 'train_form', 'fused') == 'ops' else train.tgnn_ce_fused
-            ce, logits = fwd(net, batch, adj_t, st['deg_t'], st['flags'], t_graph, row, col, tgt, pair_graph, dp)
+            args = (net, batch, adj_t, st['deg_t'], st['flags'], t_graph, row, col, tgt, pair_graph, dp)
+            ce, logits = train.tgnn_ce_forward(*args, keep8=form == 'ops8') if form in ('ops', 'ops8') else train.tgnn_ce_fused(*args)
             if not ce.requires_grad:
                 batch._train_ws_busy = False      # no backward will come to release the workspace
             npairs = batch.edges_per_graph.to(dev).float()

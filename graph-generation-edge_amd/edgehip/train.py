@@ -10,7 +10,7 @@ import ctypes as C
 import torch
 from torch.autograd import Function
 
-from . import capi
+from . import capi, ckpt8
 
 byref = C.byref
 lib = capi.lib
@@ -282,16 +282,8 @@ class _Dropout(Function):
         return dx, None, None, None
 
 
-def linear(x, m):
-    return _Linear.apply(x, m.weight, m.bias)
-
-
 def act(x, kind=SILU):
     return _Act.apply(x, kind)
-
-
-def _mlp2(x, seq):
-    return linear(act(linear(x, seq[0])), seq[2])
 
 
 def pair_targets(batch, adj_tm1, row, col):
@@ -304,41 +296,90 @@ def pair_targets(batch, adj_tm1, row, col):
     return tgt, pg
 
 
-def tgnn_ce_forward(net, batch, adj_t, deg_t, flags, t_graph, row, col, tgt, pair_graph, dp=None):
-    """Differentiable TGNN_degree_guided.forward on the active pairs (row, col) followed by the per-graph
-    cross-entropy against `tgt`.  Returns (ce_graph [B] with grad, logits [A,2])."""
+class _Ops:
+    """The layers' ops, keeping their inputs whole for the backward."""
+    linear = staticmethod(_Linear.apply)
+    act = staticmethod(act)
+
+    @staticmethod
+    def keep(x):
+        return None
+
+
+class _Ops8(_Ops):
+    """The same ops, keeping the inputs of linear layers and activations in 8 bits (ckpt8.py).  `keep` packs an input that
+    several layers read once for all of them."""
+
+    @staticmethod
+    def linear(x, w, b, kept=None):
+        return ckpt8.linear8(x, w, b, kept)
+
+    @staticmethod
+    def act(x, kind=SILU):
+        return ckpt8.act8(x, 'silu' if kind == SILU else 'mish')
+
+    @staticmethod
+    def keep(x):
+        return ckpt8.pack8(x.detach()) if torch.is_grad_enabled() else None
+
+
+def _tgnn_pair_hidden(net, batch, adj_t, deg_t, flags, t_graph, row, col, dp, ops):
+    """Differentiable TGNN_degree_guided.forward on the active pairs (row, col) up to the last layer: e2 [A,64]."""
+    def linear(x, m, kept=None):
+        return ops.linear(x, m.weight, m.bias) if kept is None else ops.linear(x, m.weight, m.bias, kept)
+
+    def mlp2(x, seq):
+        return linear(ops.act(linear(x, seq[0])), seq[2])
+
     L = batch.layout
     X0 = _Embed.apply(net.embedding_t.weight, net.embedding_t.bias, net.embedding_0.weight, net.embedding_0.bias,
                       net.embedding_sel.weight, L, deg_t, batch.degree_i32, flags, int(net.max_degree))
-    nodes0 = act(linear(X0, net.node_in[0]))                                   # layers.py:335-336
+    nodes0 = ops.act(linear(X0, net.node_in[0]))                               # layers.py:335-336
     pe = net._pos_emb.index_select(0, t_graph.long())                          # table lookup, no grad
-    mt = act(_mlp2(pe, net.mlp), MISH)                                         # layers.py:338-339, :31-34
+    mt = ops.act(mlp2(pe, net.mlp), MISH)                                      # layers.py:338-339, :31-34
     h = hid = nodes0                         # h: GRU output `nodes`; hid: the hidden state carried on (dropped, :361)
     drop = dp is not None and dp.p > 0
-    cx = _mlp2(_SegmentMean.apply(nodes0, None, L), net.global_mlp)            # layers.py:342-343
+    cx = mlp2(_SegmentMean.apply(nodes0, None, L), net.global_mlp)             # layers.py:342-343
     for i, heads in enumerate(net.num_heads):
         tl = linear(mt, net.layers[f'time{i}'].linear)
         x = _Assemble.apply(h, cx if i > 0 else None, tl, None, L)             # cat[nodes, t_emb], nodes = h + ctx
         cv = net.layers[f'conv{i}']
-        conv = _Attention.apply(linear(x, cv.lin_query), linear(x, cv.lin_key), linear(x, cv.lin_value),
-                                linear(x, cv.lin_skip), L, adj_t, heads)
-        xs = act(conv)
+        kx = ops.keep(x)
+        conv = _Attention.apply(linear(x, cv.lin_query, kx), linear(x, cv.lin_key, kx), linear(x, cv.lin_value, kx),
+                                linear(x, cv.lin_skip, kx), L, adj_t, heads)
+        xs = ops.act(conv)
         if drop:
             xs = _Dropout.apply(xs, L, dp, 2 * i)                              # :357
-        gi = _Linear.apply(xs, net.gru.weight_ih_l0, net.gru.bias_ih_l0)
-        gh = _Linear.apply(hid, net.gru.weight_hh_l0, net.gru.bias_hh_l0)
+        gi = ops.linear(xs, net.gru.weight_ih_l0, net.gru.bias_ih_l0)
+        gh = ops.linear(hid, net.gru.weight_hh_l0, net.gru.bias_hh_l0)
         h = _GruGate.apply(gi, gh, hid)
         hid = _Dropout.apply(h, L, dp, 2 * i + 1) if drop and i + 1 < len(net.num_heads) else h   # :361
         cin = _Assemble.apply(h, None, cx, None, L)                            # cat[nodes, contexts]  :366
-        nctx = _mlp2(cin, net.context_mlp)
-        cx = _mlp2(_SegmentMean.apply(nctx, cx, L), net.global_mlp)            # :367-368
+        nctx = mlp2(cin, net.context_mlp)
+        cx = mlp2(_SegmentMean.apply(nctx, cx, L), net.global_mlp)             # :367-368
     zin = _Assemble.apply(h, cx, None, X0, L)                                  # :371, :377
     no = net.node_out_mlp
-    z = linear(act(linear(act(linear(zin, no[0])), no[2])), no[4])
+    z = linear(ops.act(linear(ops.act(linear(zin, no[0])), no[2])), no[4])
     e = _PairGatherAdd.apply(z, row, col)                                      # :380
     fo = net.final_out
-    e2 = act(linear(act(linear(e, fo[0])), fo[2]))
+    return ops.act(linear(ops.act(linear(e, fo[0])), fo[2]))
+
+
+def tgnn_ce_forward(net, batch, adj_t, deg_t, flags, t_graph, row, col, tgt, pair_graph, dp=None, keep8=False):
+    """Differentiable TGNN_degree_guided.forward on the active pairs (row, col) followed by the per-graph
+    cross-entropy against `tgt`.  Returns (ce_graph [B] with grad, logits [A,2]).  keep8: what the layers keep for the
+    backward is kept in 8 bits (same loss, gradients of the weights and through the activations from the kept values)."""
+    e2 = _tgnn_pair_hidden(net, batch, adj_t, deg_t, flags, t_graph, row, col, dp, _Ops8 if keep8 else _Ops)
+    fo = net.final_out
     return _EdgeCE.apply(e2, fo[4].weight, fo[4].bias, tgt, pair_graph, batch.num_graphs)
+
+
+def tgnn_pair_logits(net, batch, adj_t, deg_t, flags, t_graph, row, col, dp=None, keep8=False):
+    """The logits [A,2] of the active pairs (row, col), differentiable: what the losses of tune.py read, with the batch's
+    active-pair offsets (`aptr`) as the sequences and the sampled bits as what was taken."""
+    e2 = _tgnn_pair_hidden(net, batch, adj_t, deg_t, flags, t_graph, row, col, dp, _Ops8 if keep8 else _Ops)
+    fo = net.final_out
+    return torch.nn.functional.linear(e2, fo[4].weight, fo[4].bias)
 
 
 # ------------------------------------------------------------------------------------------------------

@@ -475,6 +475,126 @@ int edgehip_graph_stats_ext(const edgehip_layout* L, const uint32_t* adj, int32_
 int edgehip_edge_overlap(const edgehip_layout* L, const uint32_t* adj_a, const uint32_t* adj_b, int64_t* out,
                          void* stream);
 
+/* ================================================================================================
+ * Operators for deeper networks and their tuning.  NO COUNTERPART in the reference (its network keeps
+ * fp32 activations, has no norms and one loss); they stand beside the training ops above and follow the
+ * same conventions.  Types: EDGEHIP_F32 / _BF16 / _F16; statistics, sums and gradients of parameters are
+ * held in fp32 (per-row scalars of the losses in fp64), every output is rounded once.  Rows may start at
+ * any element-aligned address.  All sums are made in a fixed order: the same input gives the same bits.
+ * ================================================================================================ */
+#define EDGEHIP_F32 0
+#define EDGEHIP_BF16 1
+#define EDGEHIP_F16 2
+
+/* ---- the step between two blocks: norms before and after, gate, residual scale -------------------
+ *   u = N_post(z);  h_out = res_scale h + gate u;  y = N_pre(h_out)
+ * N(x) = (x - mean) / sqrt(mean((x - mean)^2) + eps) * w + b over the dim values of a row (kind LAYER), or
+ * x / sqrt(mean(x^2) + eps) * w (kind RMS, no bias).  post == 0: u = z; pre == 0: there is no y.  y is the norm of the
+ * UNROUNDED h_out.  w NULL: ones, b NULL: zeros.
+ * The gate: none (1), one vector [dim], one row per group of rows [groups, dim] (group g: rows row_ptr[g] ..
+ * row_ptr[g+1]-1, row_ptr[0] = 0, ascending, empty groups allowed; node_ptr of a layout is one), or one per row
+ * [rows, dim].  Rows behind the last group have gate 0: they pass as res_scale h.
+ * h, h_out, dh*, are of stream_dtype; z, y, dz, dy of branch_dtype; stream_dtype = branch_dtype or F32.  w, b (and
+ * their gradients) are of param_dtype, the gate (and its gradient) of gate_dtype: each F32 or branch_dtype.
+ * dim <= 8192.  Buffers are dense; outputs must not overlap inputs. */
+#define EDGEHIP_NORM_RMS 0
+#define EDGEHIP_NORM_LAYER 1
+#define EDGEHIP_GATE_NONE 0
+#define EDGEHIP_GATE_VECTOR 1
+#define EDGEHIP_GATE_GROUP 2
+#define EDGEHIP_GATE_ROW 3
+typedef struct edgehip_gate_norm {
+    int64_t rows;
+    int32_t dim, stream_dtype, branch_dtype, kind, pre, post, param_dtype, gate_kind, gate_dtype, groups;
+    const void *w_pre, *b_pre, *w_post, *b_post;      /* [dim] */
+    const void* gate;
+    const int32_t* row_ptr;                           /* [groups+1], gate_kind GROUP only */
+    float res_scale, eps;
+} edgehip_gate_norm;
+/* stats [rows,4] fp32 (16-byte aligned; NULL when no backward follows): mean and 1/size of z, then of h_out. */
+int edgehip_gate_norm_fwd(const edgehip_gate_norm* G, const void* h, const void* z, void* h_out, void* y, float* stats,
+                          void* stream);
+/* The backward pass from the forward's INPUTS h and z and its stats.  dh_out / dy: gradients of the outputs (NULL: zero).
+ * dh, dz are written; dgate, dw_pre, db_pre, dw_post, db_post are OVERWRITTEN (NULL: not wanted).
+ * ws: edgehip_gate_norm_workspace_bytes(G) bytes, 16-byte aligned (0 bytes: a configuration the call would refuse). */
+size_t edgehip_gate_norm_workspace_bytes(const edgehip_gate_norm* G);
+int edgehip_gate_norm_bwd(const edgehip_gate_norm* G, const void* dh_out, const void* dy, const void* h, const void* z,
+                          const float* stats, void* dh, void* dz, void* dgate, void* dw_pre, void* db_pre, void* dw_post,
+                          void* db_post, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- activations kept for the backward pass in 8 bits ------------------------------------------------
+ * A row of K values is cut into groups of 64 (the last may be shorter).  A group keeps e, the smallest integer of
+ * [-120, 121] with max|x| <= 127 2^e (121 if there is none), and the whole numbers round-to-even(x 2^-e), held to
+ * [-127, 127]; it stands for code * 2^e.  codes [M,K] int8,
+ * exps [M, ceil(K/64)] int8.  e = -128: the group held an infinity or NaN, all of it stands for NaN.
+ * pack8 / unpack8: x of `dtype`.  act8_fwd: y = act(x) and the checkpoint of x in one pass; act8_bwd:
+ * dx = dy act'(kept x).  kind: 1 SiLU, 2 Mish (those of edgehip_act_fwd). */
+#define EDGEHIP_ACT_SILU 1
+#define EDGEHIP_ACT_MISH 2
+int edgehip_pack8(int32_t dtype, const void* x, int64_t M, int64_t K, int8_t* codes, int8_t* exps, void* stream);
+int edgehip_unpack8(int32_t dtype, const int8_t* codes, const int8_t* exps, int64_t M, int64_t K, void* x, void* stream);
+int edgehip_act8_fwd(int32_t dtype, int32_t kind, const void* x, int64_t M, int64_t K, void* y, int8_t* codes, int8_t* exps,
+                     void* stream);
+int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, const int8_t* codes, const int8_t* exps, int64_t M,
+                     int64_t K, void* dx, void* stream);
+/* The weight gradient of y = x W^T + b from the kept x: dW[N,K] = dY[M,N]^T X8[M,K], db[N] = column sums of dY (NULL: not
+ * wanted); both fp32, OVERWRITTEN.  dY of `dtype`; every product is exact, sums are fp32, in a fixed order.
+ * ws: edgehip_linear8_workspace_bytes bytes (0: a configuration the call would refuse). */
+size_t edgehip_linear8_workspace_bytes(int32_t dtype, int64_t M, int32_t N, int32_t K);
+int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const int8_t* codes, const int8_t* exps, int64_t M, int32_t N,
+                               int32_t K, float* dW, float* db, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- losses over rows of logits that tune a trained model ---------------------------------------------
+ * Row r of `logits` [rows, classes] (row_stride values from one row to the next) chose class taken[r]; sequence s is the
+ * rows seq_ptr[s] .. seq_ptr[s+1]-1 (ascending from 0; the `aptr` of the active pairs is one).  A row counts if
+ * mask[r] != 0 (mask NULL: every row), 0 <= taken[r] < classes and it lies in a sequence; the others have log-probability
+ * 0 and gradient 0 whatever their logits hold.  dlogits is dense [rows, classes], of the logits' dtype, written whole. */
+typedef struct edgehip_logit_rows {
+    int64_t rows, row_stride;
+    int32_t classes, dtype, num_seqs, reserved;
+    const void* logits;
+    const int64_t* taken;
+    const uint8_t* mask;
+    const int64_t* seq_ptr;              /* [num_seqs+1] */
+} edgehip_logit_rows;
+/* logp[r] = log softmax(logits[r])[taken[r]], fp32; num_seqs 0 and seq_ptr NULL: one sequence of all rows */
+int edgehip_row_logp(const edgehip_logit_rows* Q, float* logp, void* stream);
+/* The policy loss.  With rho = exp(logp - old_logp), A the advantage (of the sequence, or of the row), gap = ref_logp - logp:
+ *   term = -min(rho A, clip(rho, 1 - clip_lo, 1 + clip_hi) A) + kl_coef (exp(gap) - gap - 1)
+ * loss[s] = sum of the terms of its counted rows, divided by their number with `mean`; kl[s] the same of exp(gap) - gap - 1
+ * (0 without ref_logp); clipped[s]: rows where the clip binds.  A sequence without counted rows has loss 0. */
+typedef struct edgehip_policy {
+    const float *old_logp, *advantage, *ref_logp;    /* [rows], [num_seqs] or [rows], [rows] or NULL */
+    const float* weight;                 /* [num_seqs]: the gradient is that of sum weight[s] loss[s]; NULL: 1 / num_seqs each */
+    double clip_lo, clip_hi, kl_coef;
+    int32_t advantage_per_row, mean;
+} edgehip_policy;
+/* The preference loss of num_seqs / 2 pairs: sequence p was preferred to sequence p + num_seqs / 2.  margin[p] = m_p - m_{p'},
+ * m the sum (`mean`: the mean) over counted rows of logp - ref_logp.
+ *   SIGMOID: loss = -(1 - label_smoothing) ln sigmoid(beta margin) - label_smoothing ln sigmoid(-beta margin)
+ *   SQUARE:  loss = (margin - 1 / (2 beta))^2 */
+#define EDGEHIP_PREFER_SIGMOID 0
+#define EDGEHIP_PREFER_SQUARE 1
+typedef struct edgehip_preference {
+    const float* ref_logp;               /* [rows] or NULL (0) */
+    const float* weight;                 /* [num_seqs / 2]; NULL: 2 / num_seqs each */
+    double beta, label_smoothing;
+    int32_t kind, mean;
+} edgehip_preference;
+/* ws: edgehip_tune_workspace_bytes(Q) bytes, 16-byte aligned.  *_fwd leaves in it what *_bwd (same arguments, weight: the
+ * gradients of the losses) needs; policy_loss_grad makes loss and gradient in one pass over the logits.  logp: [rows] or NULL. */
+size_t edgehip_tune_workspace_bytes(const edgehip_logit_rows* Q);
+int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehip_policy* O, float* loss, float* kl, int32_t* clipped,
+                            float* logp, void* ws, size_t ws_bytes, void* stream);
+int edgehip_policy_loss_bwd(const edgehip_logit_rows* Q, const edgehip_policy* O, void* dlogits, void* ws, size_t ws_bytes,
+                            void* stream);
+int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgehip_policy* O, float* loss, float* kl, int32_t* clipped,
+                             float* logp, void* dlogits, void* ws, size_t ws_bytes, void* stream);
+int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const edgehip_preference* O, float* loss, float* margin, void* ws,
+                                size_t ws_bytes, void* stream);
+int edgehip_preference_loss_bwd(const edgehip_logit_rows* Q, const edgehip_preference* O, void* dlogits, void* ws,
+                                size_t ws_bytes, void* stream);
+
 /* ---- measurement hooks (no counterpart in the reference; used by bench.py's roofline leg) -------
  * When enabled, every kernel launch of the path is bracketed by HIP events on its launch stream.
  * collect() synchronises on those events and returns, per kernel class, the summed device time (ms)

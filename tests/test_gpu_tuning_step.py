@@ -1,0 +1,139 @@
+"""GPU: the operators for deeper networks and tuning as they are used together, and in this package's own paths."""
+import numpy as np
+import pytest
+import torch
+
+import cases
+import helpers as H
+from oracle import edge_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+
+def block64(p, h, z, row_ptr, kept=None):
+    """Norm, two layers with an activation between, gated back into the stream, in fp64.  kept: the 8-bit values the
+    layers' inputs are replaced by where only their gradient reads them."""
+    def norm(x, w):
+        return x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+    own = torch.repeat_interleave(torch.arange(len(row_ptr) - 1, device=h.device), (row_ptr[1:] - row_ptr[:-1]).long())
+    h = 0.9 * h + p['gate'][own] * norm(z, p['w_post'])
+    return h, norm(h, p['w_pre'])
+
+
+def test_a_tuning_step_of_a_two_layer_block():
+    """Stream -> gated norms -> linear8 -> act8 -> linear8 -> logits -> policy loss, forward and backward, against the same
+    step in fp64 with exact inputs everywhere: the loss to fp32, the gradients to what 8-bit checkpoints leave of them -
+    a kept value is off by at most 1/127 of the largest of its 64, uniformly distributed, rms 1/127/sqrt(12) x 4 sigma: under
+    1 % of the rms; a gradient reads one checkpoint in each of two layers: 3 % of its norm."""
+    import edgehip
+    g = torch.Generator(device='cuda').manual_seed(3)
+    rows, dim, hid, seqs = 900, 128, 256, 12
+    n = lambda *s: torch.randn(*s, generator=g, device='cuda')
+    cut = torch.randint(0, rows, (seqs - 1,), generator=g, device='cuda').sort().values
+    ptr = torch.cat([cut.new_zeros(1), cut, cut.new_full((1,), rows)])
+    p = dict(w_pre=1 + 0.1 * n(dim), w_post=1 + 0.1 * n(dim), gate=0.5 + 0.2 * n(seqs, dim), w1=n(hid, dim) * dim ** -0.5, b1=0.1 * n(hid),
+             w2=n(64, hid) * hid ** -0.5, b2=0.1 * n(64))
+    h, z = n(rows, dim), n(rows, dim)
+    taken = torch.randint(0, 64, (rows,), generator=g, device='cuda')
+    mask = torch.rand(rows, generator=g, device='cuda') > 0.1
+    adv = n(seqs)
+    d = {k: v.double().requires_grad_(True) for k, v in dict(p, h=h, z=z).items()}
+    _, y = block64(d, d['h'], d['z'], ptr)
+    logits = torch.nn.functional.silu(y @ d['w1'].t() + d['b1']) @ d['w2'].t() + d['b2']
+    lp = torch.log_softmax(logits, 1).gather(1, taken[:, None])[:, 0]
+    drift = (0.2 * n(rows)).double()
+    old = (lp.detach() - drift).float()
+    rho = torch.exp(lp - old.double())
+    own = torch.repeat_interleave(torch.arange(seqs, device='cuda'), ptr[1:] - ptr[:-1])
+    A = adv.double()[own]
+    each = -torch.minimum(rho * A, rho.clamp(0.8, 1.2) * A) * mask
+    total = torch.zeros(seqs, dtype=torch.float64, device='cuda').index_add(0, own, each)
+    count = torch.zeros(seqs, dtype=torch.float64, device='cuda').index_add(0, own, mask.double()).clamp_min(1)
+    want_loss = total / count
+    want = torch.autograd.grad(want_loss.mean(), list(d.values()))
+
+    leaves = {k: v.clone().requires_grad_(True) for k, v in dict(p, h=h, z=z).items()}
+    _, y = edgehip.gate_norm(leaves['h'], leaves['z'], w_pre=leaves['w_pre'], w_post=leaves['w_post'], gate=leaves['gate'],
+                             row_ptr=ptr.to(torch.int32), res_scale=0.9)
+    x = edgehip.linear8(edgehip.act8(edgehip.linear8(y, leaves['w1'], leaves['b1'])), leaves['w2'], leaves['b2'])
+    out = edgehip.policy_loss(x, taken, old, adv, ptr, mask=mask)
+    got = torch.autograd.grad(out.loss.mean(), list(leaves.values()), retain_graph=True)
+    assert bool(((out.loss.double() - want_loss).abs() <= 1e-4 * (1 + want_loss.abs())).all())
+    for k, a, b in zip(leaves, got, want):
+        assert float((a.double() - b).norm()) <= 0.03 * float(b.norm()), k
+    # the gradient made with the loss, handed on, is the same step
+    r = edgehip.policy_loss_grad(x.detach(), taken, old, adv, ptr, mask=mask)
+    more = torch.autograd.grad(x, list(leaves.values()), r.dlogits)
+    for k, a, b in zip(leaves, got, more):
+        assert float((a - b).norm()) <= 1e-5 * float(a.norm()), k
+
+
+def _step(form, graphs, T, params, seed=2):
+    model = H.build_model(params, T, cases.max_degree_of(graphs))
+    model.train()
+    model.train_form = form
+    b = H.graph_batch(graphs, degree_dtype=np.int64)
+    gen = torch.Generator().manual_seed(seed)
+    t = torch.full((len(graphs),), T // 3)
+    pairs = sum(q['n'] * (q['n'] - 1) // 2 for q in graphs)
+    u1, u3 = torch.rand(pairs, 2, generator=gen).cuda(), torch.rand(pairs, 2, generator=gen).cuda()
+    nv = model.log_prob(b, t, torch.full((len(graphs),), 1.0 / T), u1, u3)
+    (-nv.sum() / (np.log(2) * b.num_entries)).backward()
+    return model, b, nv.detach(), {k: v.grad.detach().clone() for k, v in model._denoise_fn.named_parameters() if v.grad is not None}
+
+
+def test_the_training_form_with_8_bit_checkpoints():
+    """train_form 'ops8' computes the loss of 'ops' (the same kernels on the same inputs); its gradients read inputs that are
+    off by under 1 % of a group's rms (see above) in each of the ~20 layers between a weight and the loss: 10 % of each."""
+    graphs = cases.ragged_graphs(5) + cases.ragged_graphs(6)
+    params = orc.random_tgnn_params(4)
+    _, _, nv, ref = _step('ops', graphs, 48, params)
+    _, _, nv8, got = _step('ops8', graphs, 48, params)
+    assert torch.allclose(nv, nv8, rtol=1e-6, atol=1e-9)
+    assert set(ref) == set(got)
+    gmax = max(float(g.norm()) for g in ref.values())
+    for k in ref:
+        assert float((ref[k] - got[k]).norm()) <= 0.1 * max(float(ref[k].norm()), 1e-3 * gmax), k
+
+
+def test_tuning_the_graph_sampler_on_its_own_decisions():
+    """The active pairs of a batch, what was taken there and `aptr` go into the policy loss: the network's gradient is that
+    of the formula in fp64 on the same logits (5e-7 relative each, the backward kernels' own bound 2e-4), with whole and -
+    within the bound above - with 8-bit checkpoints."""
+    import edgehip
+    from edgehip import train
+    from edgehip.model import _state
+    graphs = cases.ragged_graphs(5)
+    model, b, _, _ = _step('ops', graphs, 48, orc.random_tgnn_params(4))
+    net, st = model._denoise_fn, _state(b)
+    t_graph = torch.full((b.num_graphs,), 16, dtype=torch.int32, device='cuda')
+    row, col = b.active_row, b.active_col
+    assert row.numel() > 50
+    adv = torch.randn(b.num_graphs, device='cuda')
+    taken = torch.randint(0, 2, (row.numel(),), device='cuda')
+    n = st['aptr'][1:] - st['aptr'][:-1]
+    own = torch.repeat_interleave(torch.arange(b.num_graphs, device='cuda'), n)
+
+    def gradients(loss):
+        net.zero_grad()
+        loss.backward()
+        return {k: p.grad.clone() for k, p in net.named_parameters() if p.grad is not None}
+    ask = lambda keep8: train.tgnn_pair_logits(net, b, b.adj, st['deg_t'], st['flags'], t_graph, row, col, keep8=keep8)
+    logits = ask(False)
+    old = edgehip.row_logp(logits.detach(), taken) - 0.1
+    out = edgehip.policy_loss(logits, taken, old, adv, st['aptr'])
+    got = gradients(out.loss.sum())
+    logits = ask(False)
+    lp = torch.log_softmax(logits.double(), 1).gather(1, taken[:, None])[:, 0]
+    rho = torch.exp(lp - old.double())
+    each = -torch.minimum(rho * adv.double()[own], rho.clamp(0.8, 1.2) * adv.double()[own]) / n[own]
+    loss = torch.zeros(b.num_graphs, dtype=torch.float64, device='cuda').index_add(0, own, each)
+    assert bool(((out.loss.double() - loss).abs() <= 1e-6 * (1 + loss.abs())).all())
+    want = gradients(loss.sum())
+    kept = gradients(edgehip.policy_loss(ask(True), taken, old, adv, st['aptr']).loss.sum())
+    assert set(got) == set(want) == set(kept) and len(got) > 80
+    gmax = max(float(g.norm()) for g in want.values())
+    for k, g in want.items():
+        size = float(g.norm())
+        assert float((got[k] - g).norm()) <= 2e-4 * max(size, 1e-3 * gmax), k
+        assert float((kept[k] - g).norm()) <= 0.1 * max(size, 1e-3 * gmax), k
