@@ -205,29 +205,38 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 // ------------------------------------------------------------------------------------------------------------------
 // dW[N][K] = dY[M][N]^T X8[M][K], db[n] = sum over m of dY[m][n].
 //
-// The sum runs over the ROWS of both operands, the slow axis of both: a matrix instruction wants eight consecutive m of
-// one column per lane.  A thread therefore stages an 8 x 8 block (eight rows, eight columns: 16-byte reads of 16-bit
-// rows), turns it in registers - two rows' values of a column side by side are one v_perm - and writes eight 16-byte
-// pieces [column][eight m] to LDS.  Tile image: piece (m / 8, column c) at ((m / 8) * 128 + c') * 16 bytes, c' = c with
-// its low three bits xored by the next three: the eight writers of a bank phase hold columns 8 apart and land in eight
-// different 16-byte slots, and a fragment (32 consecutive columns) still reads 32 consecutive pieces.
+// The sum runs over the ROWS of both operands, the slow axis of both, while a matrix instruction wants eight consecutive
+// m of one column in a lane.  A thread therefore stages an 8-row x CW-column piece of each operand (16-byte reads of a
+// 16-bit dY), turns it in registers - two rows' values of a column side by side are one v_perm - and writes CW 16-byte
+// pieces [column][eight m] to LDS.  The piece (m / 8, column c) stands at ((m / 8) T + c') 16 bytes, c' = c with its low
+// three bits xored by the next three: the eight writers of a bank phase, whose columns are 4 or 8 apart, land in eight
+// different slots, and a fragment (32 consecutive columns) still reads 32 consecutive pieces: no bank conflicts.
 //
-// A block owns a 128 x 128 tile of dW and a run of rows (blockIdx.z); four waves, 64 x 64 each.  The rows are split
-// when the tiles alone do not fill the chip; partial tiles go to the workspace and are added in order by k_ck_dw_sum.
+// A block owns a T x T tile of dW and a run of rows; four waves, T/2 x T/2 each.  T = 256: 64 (T = 128: 32) bytes are read
+// from LDS per matrix instruction and lane half... the larger tile needs half the LDS reads per flop and is taken where the
+// matrix pipe is the bound.  Two LDS images: while a chunk of BM rows is multiplied, the next one's registers (requested
+// a chunk earlier) are turned and written, and the one after is requested; one barrier a chunk, which waits for LDS
+// only, so that the requests stay in flight across it.
+//
+// The rows are split where the tiles alone do not fill the chip; partial tiles go to the workspace and are added in
+// order by k_ck_dw_sum.  db: the block of k-tile j adds up the chunks with number j modulo the k-tiles, so that this work
+// is spread over them; partials by (split, k-tile).
 // ------------------------------------------------------------------------------------------------------------------
-#define DW_T 128
-#define DW_M 32
-#define DW_PIECES (DW_M / 8 * DW_T)          // 16-byte pieces of one operand plane
+#define CK_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
 template <int DT> struct dw_planes { static constexpr int value = DT == EDGEHIP_BF16 ? 1 : DT == EDGEHIP_F16 ? 2 : 3; };
+// rows a chunk: two images of (planes + 1) x T x BM x 2 bytes must fit the 160 KB of LDS
+template <int DT, int T> struct dw_rows { static constexpr int value = T == 256 && DT != EDGEHIP_BF16 ? 32 : 64; };
 
 // x = t[0] + t[1] + ... by truncation to 8 significant bits each; the upper halves of two rows' values in one dword.
-// An infinity or NaN stays in the first term (its remainder would be NaN: zero instead).
+// An infinity or NaN stays in the first term (its remainder would be NaN: zero instead); a NaN whose payload lies in
+// the low half is made quiet first, truncation would turn it into an infinity.
 template <int P>
 __device__ static inline void dw_split(float x0, float x1, unsigned (&o)[P]) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const unsigned u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+        unsigned u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+        if (p == 0 && P > 1) { u0 = x0 != x0 ? 0x7fc00000u : u0; u1 = x1 != x1 ? 0x7fc00000u : u1; }
         o[p] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
         if (p + 1 < P) {
             x0 = (u0 & 0x7f800000u) == 0x7f800000u ? 0.0f : x0 - __uint_as_float(u0 & 0xffff0000u);
@@ -235,156 +244,294 @@ __device__ static inline void dw_split(float x0, float x1, unsigned (&o)[P]) {
         }
     }
 }
-// (truncation would turn a NaN whose payload lies in the low half into an infinity: such values are made quiet first)
-__device__ static inline float dw_quiet(float x) { return x != x ? __uint_as_float(0x7fc00000u) : x; }
 
-__device__ static inline int dw_piece(int mblk, int c) { return mblk * DW_T + ((c & ~7) | ((c ^ (c >> 3)) & 7)); }
+template <int T>
+__device__ static inline int dw_piece(int mblk, int c) { return mblk * T + ((c & ~7) | ((c ^ (c >> 3)) & 7)); }
 
-template <int DT>
-__global__ __launch_bounds__(256) void k_ck_dw(const void* __restrict__ dY, const int8_t* __restrict__ codes, const int8_t* __restrict__ exps,
-                                               int64_t M, int N, int K, int KG, int64_t rows_per_split, float* __restrict__ out,
-                                               float* __restrict__ db) {
-    constexpr int P = dw_planes<DT>::value;
-    __shared__ ck_u32x4 ya[P][DW_PIECES], xa[DW_PIECES];
+// CW consecutive values of a dY row as they stand in memory: DWORDS registers
+template <int DT, int CW> struct dw_y {
+    static constexpr int DWORDS = CW * (DT == EDGEHIP_F32 ? 4 : 2) / 4;
+    unsigned d[DWORDS];
+    __device__ inline void load(const char* p) {
+        typedef unsigned vec __attribute__((ext_vector_type(DWORDS), aligned(2)));
+        const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int i = 0; i < DWORDS; ++i) d[i] = v[i];
+    }
+    __device__ inline void load_some(const char* p, int n) {             // n < CW of them, zeros behind
+#pragma unroll
+        for (int i = 0; i < DWORDS; ++i) d[i] = 0u;
+#pragma unroll
+        for (int c = 0; c < CW; ++c) {
+            if (c >= n) continue;
+            if (DT == EDGEHIP_F32) d[c < DWORDS ? c : 0] = reinterpret_cast<const unsigned*>(p)[c];
+            else d[c / 2 < DWORDS ? c / 2 : 0] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[c] << (16 * (c & 1));
+        }
+    }
+    __device__ inline float get(int c) const {
+        if (DT == EDGEHIP_F32) return __uint_as_float(d[c < DWORDS ? c : 0]);
+        const unsigned w = d[c / 2 < DWORDS ? c / 2 : 0];
+        if (DT == EDGEHIP_BF16) return __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16);
+        return (float)__builtin_bit_cast(_Float16, (unsigned short)(c & 1 ? w >> 16 : w));
+    }
+};
+
+template <int DT, int T>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __restrict__ dY, const int8_t* __restrict__ codes,
+                                                                const int8_t* __restrict__ exps, int64_t M, int N, int K, int KG,
+                                                                int64_t rows_per_split, int nt, int kt, float* __restrict__ out,
+                                                                float* __restrict__ db) {
+    constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT, T>::value, CW = T * BM / 2048, W = T / 2, F = W / 32;
+    constexpr int PIECES = BM / 8 * T, ES = DT == EDGEHIP_F32 ? 4 : 2;
+    __shared__ ck_u32x4 img[2][(P + 1) * PIECES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int k0 = blockIdx.x * DW_T, n0 = blockIdx.y * DW_T;
-    const int64_t m0 = (int64_t)blockIdx.z * rows_per_split;
+    // tiles in runs of four n-tiles; consecutive tiles to one XCD (blocks are dealt to the eight of them in turn), so that
+    // its L2 holds the few panels its blocks share
+    int id = blockIdx.x;
+    const int total = nt * kt;
+    if ((total & 7) == 0) id = (id & 7) * (total >> 3) + (id >> 3);
+    const int band = id / (4 * kt), left = nt - band * 4 < 4 ? nt - band * 4 : 4, in = id - band * 4 * kt;
+    const int n0 = (band * 4 + in % left) * T, ktile = in / left, k0 = ktile * T;
+    const int64_t m0 = (int64_t)blockIdx.y * rows_per_split;
     const int64_t m1 = m0 + rows_per_split < M ? m0 + rows_per_split : M;
-    // staging: threads 0..63 the 8x8 blocks of dY, 64..127 those of X (4 x 16 blocks each)
-    const int c8 = (lane & 15) * 8, mb = lane >> 4;
-    const bool want_db = db && blockIdx.x == 0;
-    float bsum[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bsum[i] = 0.0f;
-    ck_f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    const int wn = (wave & 1) * 64, wk = (wave >> 1) * 64;
-    for (int64_t m = m0; m < m1; m += DW_M) {
-        __syncthreads();
-        if (wave < 2) {
-            float v[8][8];
-            const int64_t r = m + mb * 8;
+    // staging: this thread's columns and eight rows of both operands
+    const int c0 = (tid % (T / CW)) * CW, mb = tid / (T / CW);
+    const char* yp = reinterpret_cast<const char*>(dY) + (m0 + mb * 8) * (int64_t)N * ES + (int64_t)(n0 + c0) * ES;
+    const int8_t* xp = codes + (m0 + mb * 8) * (int64_t)K + k0 + c0;
+    const int8_t* ep = exps + (m0 + mb * 8) * (int64_t)KG + ((k0 + c0) >> 6);
+    const int ny = N - n0 - c0, nx = K - k0 - c0;
+    const bool inner = n0 + T <= N && k0 + T <= K;
+    dw_y<DT, CW> y[8];
+    unsigned x[8][CW / 4];
+    int e[8];
+    auto request = [&](int64_t m) {
+        const int64_t r0 = m + mb * 8;
+        if (inner && m + BM <= m1) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool in = r + i < m1;
-                if (wave == 0) {
-                    eh_load8<DT>(dY, (r + i) * N + n0 + c8, in ? N - n0 - c8 : 0, v[i]);
-                } else {
-                    const int n = K - k0 - c8;
-                    const float st = in && n > 0 ? ck_step(exps[(r + i) * KG + ((k0 + c8) >> 6)]) : 0.0f;
-                    ck_load_codes(codes, (r + i) * K + k0 + c8, in ? n : 0, st, v[i]);
-                }
+                y[i].load(yp + (int64_t)i * N * ES);
+                typedef unsigned vec __attribute__((ext_vector_type(CW / 4), aligned(1)));
+                const vec v = *reinterpret_cast<const vec*>(xp + (int64_t)i * K);
+#pragma unroll
+                for (int j = 0; j < CW / 4; ++j) x[i][j] = v[j];
+                e[i] = ep[(int64_t)i * KG];
             }
-            if (wave == 0) {
-                if (want_db) {
+        } else {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
+            for (int i = 0; i < 8; ++i) {
+                const bool live = r0 + i < m1;
+                if (live && ny >= CW) y[i].load(yp + (int64_t)i * N * ES);
+                else y[i].load_some(yp + (int64_t)i * N * ES, live ? ny : 0);
+                e[i] = 0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) bsum[c] += v[i][c];
-                }
+                for (int j = 0; j < CW / 4; ++j) x[i][j] = 0u;
+                if (live && nx > 0) {
+                    e[i] = ep[(int64_t)i * KG];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    ck_u32x4 w[P];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        unsigned o[P];
-                        dw_split<P>(dw_quiet(v[2 * i][c]), dw_quiet(v[2 * i + 1][c]), o);
-#pragma unroll
-                        for (int p = 0; p < P; ++p) w[p][i] = o[p];
-                    }
-#pragma unroll
-                    for (int p = 0; p < P; ++p) ya[p][dw_piece(mb, c8 + c)] = w[p];
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    ck_u32x4 w;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        unsigned o[1];
-                        dw_split<1>(v[2 * i][c], v[2 * i + 1][c], o);
-                        w[i] = o[0];
-                    }
-                    xa[dw_piece(mb, c8 + c)] = w;
+                    for (int c = 0; c < CW; ++c)
+                        if (c < nx) x[i][c / 4] |= ((unsigned)xp[(int64_t)i * K + c] & 0xffu) << (8 * (c & 3));
                 }
             }
         }
-        __syncthreads();
+        yp += (int64_t)BM * N * ES;
+        xp += (int64_t)BM * K;
+        ep += (int64_t)BM * KG;
+    };
+    float bsum[CW];
 #pragma unroll
-        for (int s = 0; s < DW_M / 16; ++s) {
-            const int mblk = s * 2 + (lane >> 5);
-            ck_bf16x8 b[2];
+    for (int c = 0; c < CW; ++c) bsum[c] = 0.0f;
+    auto put_y = [&](ck_u32x4* im, int ca, int cb) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) b[j] = __builtin_bit_cast(ck_bf16x8, xa[dw_piece(mblk, wk + j * 32 + (lane & 31))]);
+        for (int c = ca; c < cb; ++c) {
+            ck_u32x4 w[P];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unsigned o[P];
+                if (DT == EDGEHIP_BF16) o[0] = __builtin_amdgcn_perm(y[2 * i + 1].d[c / 2], y[2 * i].d[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                else dw_split<P>(y[2 * i].get(c), y[2 * i + 1].get(c), o);
+#pragma unroll
+                for (int p = 0; p < P; ++p) w[p][i] = o[p];
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) im[p * PIECES + dw_piece<T>(mb, c0 + c)] = w[p];
+        }
+    };
+    auto put_x = [&](ck_u32x4* im, int ca, int cb) {
+        float st[8], off[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // exponent -128 gives -infinity, and such a group's codes are 0: code * step is NaN, as it should be
+            st[i] = __uint_as_float((unsigned)(127 + e[i]) << 23);
+            off[i] = -128.0f * st[i];
+        }
+#pragma unroll
+        for (int c = ca; c < cb; ++c) {
+            ck_u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // code + 128 as an unsigned byte, times the step, minus 128 steps: both exact
+                    const unsigned b = ((x[2 * i + h][c / 4] ^ 0x80808080u) >> (8 * (c & 3))) & 0xffu;
+                    v[h] = __builtin_fmaf((float)b, st[2 * i + h], off[2 * i + h]);
+                }
+                w[i] = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
+            }
+            im[P * PIECES + dw_piece<T>(mb, c0 + c)] = w;
+        }
+    };
+    ck_f32x16 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    const int wn = (wave & 1) * W, wk = (wave >> 1) * W, fr = lane & 31, fh = lane >> 5;
+    int turn = 0, chunk = 0;
+    auto count_db = [&]() {
+        if (db && chunk % kt == ktile) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < CW; ++c) bsum[c] += y[i].get(c);
+        }
+        ++chunk;
+    };
+    if (m0 < m1) {
+        request(m0);
+        count_db();
+        put_y(img[0], 0, CW);
+        put_x(img[0], 0, CW);
+        if (m0 + BM < m1) request(m0 + BM);
+    }
+    for (int64_t m = m0; m < m1; m += BM) {
+        CK_BARRIER();
+        const bool more = m + BM < m1;
+        const ck_u32x4* im = img[turn];
+        ck_u32x4* next = img[turn ^ 1];
+        constexpr int S = BM / 16;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int mblk = s * 2 + fh;
+            ck_bf16x8 b[F];
+#pragma unroll
+            for (int j = 0; j < F; ++j) b[j] = __builtin_bit_cast(ck_bf16x8, im[P * PIECES + dw_piece<T>(mblk, wk + j * 32 + fr)]);
 #pragma unroll
             for (int p = P - 1; p >= 0; --p) {                  // small terms first
+                ck_bf16x8 a[F];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const ck_bf16x8 a = __builtin_bit_cast(ck_bf16x8, ya[p][dw_piece(mblk, wn + i * 32 + (lane & 31))]);
+                for (int i = 0; i < F; ++i) a[i] = __builtin_bit_cast(ck_bf16x8, im[p * PIECES + dw_piece<T>(mblk, wn + i * 32 + fr)]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-                }
+                for (int i = 0; i < F; ++i)
+#pragma unroll
+                    for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+            }
+            if (more) {
+                if (s == 0) count_db();
+                put_y(next, s * CW / S, (s + 1) * CW / S);
+                put_x(next, s * CW / S, (s + 1) * CW / S);
             }
         }
+        if (more && m + 2 * BM < m1) request(m + 2 * BM);
+        turn ^= 1;
     }
-    float* o = out + (int64_t)blockIdx.z * N * K;
+    float* o = out + (int64_t)blockIdx.y * N * K;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < F; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int n = n0 + wn + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), k = k0 + wk + j * 32 + (lane & 31);
+                const int n = n0 + wn + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh, k = k0 + wk + j * 32 + fr;
                 if (n < N && k < K) o[(int64_t)n * K + k] = acc[i][j][r];
             }
-    if (want_db && wave == 0) {
+    if (db) {
+        // the BM / 8 threads that hold one column's sums, through LDS
+        __syncthreads();
+        float* red = reinterpret_cast<float*>(img[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            bsum[c] += __shfl_xor(bsum[c], 16, 64);
-            bsum[c] += __shfl_xor(bsum[c], 32, 64);
-            if (lane < 16 && n0 + c8 + c < N) db[(int64_t)blockIdx.z * N + n0 + c8 + c] = bsum[c];
+        for (int c = 0; c < CW; ++c) red[mb * T + c0 + c] = bsum[c];
+        __syncthreads();
+        if (tid < T && n0 + tid < N) {
+            float s = 0.0f;
+#pragma unroll
+            for (int b = 0; b < BM / 8; ++b) s += red[b * T + tid];
+            db[((int64_t)blockIdx.y * kt + ktile) * N + n0 + tid] = s;
         }
     }
 }
 
-// sum of the splits' partial results, in order
-__global__ __launch_bounds__(256) void k_ck_dw_sum(const float* __restrict__ part, int64_t n, int splits, float* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float a = 0.0f;
-    for (int z = 0; z < splits; ++z) a += part[z * n + i];
-    out[i] = a;
+// Sums of the partial results, in order: 64 columns of four x 16 strips of partials a block; the strips meet in LDS.  The
+// first `blocks` blocks add the tiles, the rest db.
+__global__ __launch_bounds__(1024) void k_ck_dw_sum(const float* __restrict__ part, int64_t n, int parts, float* __restrict__ out,
+                                                    const float* __restrict__ part_b, int64_t nb, int parts_b, float* __restrict__ out_b,
+                                                    int blocks) {
+    __shared__ float s[16][256 + 16];
+    const bool second = (int)blockIdx.x >= blocks;
+    const float* src = second ? part_b : part;
+    const int64_t len = second ? nb : n, at = ((int64_t)blockIdx.x - (second ? blocks : 0)) * 256 + (threadIdx.x & 63) * 4;
+    const int np = second ? parts_b : parts, strip = threadIdx.x >> 6;
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int left = at < len ? (len - at < 4 ? (int)(len - at) : 4) : 0;
+#pragma unroll 4
+    for (int z = strip; z < np; z += 16) {
+        const float* p = src + z * len + at;
+        if (left == 4) {
+            const eh_f32x4u v = *reinterpret_cast<const eh_f32x4u*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] += v[i];
+        } else {
+            for (int i = 0; i < left; ++i) a[i] += p[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[strip][(threadIdx.x & 63) * 4 + i] = a[i];
+    __syncthreads();
+    const int c = threadIdx.x;
+    const int64_t col = ((int64_t)blockIdx.x - (second ? blocks : 0)) * 256 + c;
+    if (c < 256 && col < len) {
+        float v = 0.0f;
+#pragma unroll
+        for (int z = 0; z < 16; ++z) v += s[z][c];
+        (second ? out_b : out)[col] = v;
+    }
 }
 
-// Splits of the rows: enough blocks for the 256 CUs, but at least 256 rows a split
-static int dw_splits(int64_t M, int N, int K, int64_t& rows) {
-    const int64_t tiles = (int64_t)eh_cdiv(N, DW_T) * eh_cdiv(K, DW_T);
-    int64_t s = (512 + tiles - 1) / tiles;
-    const int64_t most = (M + 255) / 256;
+struct dw_plan { int tile, nt, kt, splits; int64_t rows; };
+// The tile and the splits of the rows: one block a CU fills the chip, a split has at least 256 rows
+static dw_plan dw_choose(int64_t M, int N, int K) {
+    dw_plan p;
+    p.tile = N > 128 && K > 128 ? 256 : 128;
+    p.nt = eh_cdiv(N, p.tile);
+    p.kt = eh_cdiv(K, p.tile);
+    const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 255) / 256;
+    int64_t s = tiles >= 256 ? 1 : 256 / tiles;
     if (s > most) s = most;
     if (s < 1) s = 1;
-    rows = (M + s - 1) / s;
-    rows = (rows + DW_M - 1) / DW_M * DW_M;
-    if (rows < DW_M) rows = DW_M;
-    return (int)((M + rows - 1) / rows > 0 ? (M + rows - 1) / rows : 1);
+    p.rows = ((M + s - 1) / s + 63) / 64 * 64;
+    if (p.rows < 64) p.rows = 64;
+    p.splits = (int)((M + p.rows - 1) / p.rows);
+    if (p.splits < 1) p.splits = 1;
+    return p;
 }
 
 static int dw_check(int32_t dtype, int64_t M, int32_t N, int32_t K) {
     EH_CHECK_ARG(eh_dtype_ok(dtype) && M >= 0 && N >= 1 && K >= 1);
-    if (N > (1 << 22) || K > (1 << 22)) return EDGEHIP_ERR_TOO_LARGE;        // grid limits and 32-bit column arithmetic
+    if (N > (1 << 22) || K > (1 << 22)) return EDGEHIP_ERR_TOO_LARGE;        // 32-bit column arithmetic
     return EDGEHIP_OK;
+}
+
+static size_t dw_floats(const dw_plan& p, int N, int K, size_t& db_at) {
+    db_at = p.splits > 1 ? (size_t)p.splits * N * K : 0;
+    return db_at + (p.splits * p.kt > 1 ? (size_t)p.splits * p.kt * N : 0);
 }
 
 extern "C" size_t edgehip_linear8_workspace_bytes(int32_t dtype, int64_t M, int32_t N, int32_t K) {
     if (dw_check(dtype, M, N, K) != EDGEHIP_OK) return 0;
-    int64_t rows;
-    const int s = dw_splits(M, N, K, rows);
-    return s > 1 ? (size_t)s * ((size_t)N * K + N) * sizeof(float) : 16;
+    size_t at;
+    return dw_floats(dw_choose(M, N, K), N, K, at) * sizeof(float) + 16;
 }
 
 extern "C" int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const int8_t* codes, const int8_t* exps, int64_t M, int32_t N,
@@ -393,28 +540,31 @@ extern "C" int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const i
     if (rc != EDGEHIP_OK) return rc;
     EH_CHECK_ARG(dW && (M == 0 || (dY && codes && exps)));
     if (ws_bytes < edgehip_linear8_workspace_bytes(dtype, M, N, K)) return EDGEHIP_ERR_WORKSPACE;
-    int64_t rows;
-    const int splits = dw_splits(M, N, K, rows);
-    EH_CHECK_ARG(splits == 1 || (ws && ((uintptr_t)ws & 3) == 0));
+    const dw_plan p = dw_choose(M, N, K);
+    size_t at;
+    const size_t need = dw_floats(p, N, K, at);
+    EH_CHECK_ARG(need == 0 || (ws && ((uintptr_t)ws & 3) == 0));
     hipStream_t s = eh_stream(stream);
-    float* part = splits > 1 ? reinterpret_cast<float*>(ws) : dW;
-    float* pdb = !db ? nullptr : splits > 1 ? part + (int64_t)splits * N * K : db;
-    const dim3 grid(eh_cdiv(K, DW_T), eh_cdiv(N, DW_T), splits), block(256);
+    float* base = reinterpret_cast<float*>(ws);
+    const bool many_b = p.splits * p.kt > 1;
+    float* part = p.splits > 1 ? base : dW;
+    float* pdb = !db ? nullptr : many_b ? base + at : db;
+    const dim3 grid(p.nt * p.kt, p.splits), block(256);
     const int KG = (K + CK_GROUP - 1) / CK_GROUP;
-#define DW_GO(DT) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw<DT>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, rows, part, pdb))
-    if (dtype == EDGEHIP_F32) DW_GO(EDGEHIP_F32);
-    else if (dtype == EDGEHIP_BF16) DW_GO(EDGEHIP_BF16);
-    else DW_GO(EDGEHIP_F16);
+#define DW_GO(DT, T) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw<DT, T>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, p.nt, p.kt, part, pdb))
+#define DW_TILE(DT) do { if (p.tile == 256) DW_GO(DT, 256); else DW_GO(DT, 128); } while (0)
+    if (dtype == EDGEHIP_F32) DW_TILE(EDGEHIP_F32);
+    else if (dtype == EDGEHIP_BF16) DW_TILE(EDGEHIP_BF16);
+    else DW_TILE(EDGEHIP_F16);
+#undef DW_TILE
 #undef DW_GO
     EH_LAUNCH_CHECK();
-    if (splits > 1) {
-        const int64_t n = (int64_t)N * K;
-        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_ck_dw_sum, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, part, n, splits, dW));
+    const int64_t n = (int64_t)N * K;
+    const int blocks = p.splits > 1 ? eh_cdiv(n, 256) : 0, more = db && many_b ? eh_cdiv(N, 256) : 0;
+    if (blocks + more) {
+        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_ck_dw_sum, dim3(blocks + more), dim3(1024), 0, s, part, n, p.splits, dW, pdb, (int64_t)N,
+                                                  p.splits * p.kt, db, blocks));
         EH_LAUNCH_CHECK();
-        if (db) {
-            EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_ck_dw_sum, dim3((N + 255) / 256), dim3(256), 0, s, pdb, (int64_t)N, splits, db));
-            EH_LAUNCH_CHECK();
-        }
     }
     return EDGEHIP_OK;
 }
