@@ -245,6 +245,8 @@ __device__ static inline void dw_split(float x0, float x1, unsigned (&o)[P]) {
     }
 }
 
+template <bool B> struct dw_flag { static constexpr bool value = B; };
+
 template <int T>
 __device__ static inline int dw_piece(int mblk, int c) { return mblk * T + ((c & ~7) | ((c ^ (c >> 3)) & 7)); }
 
@@ -406,36 +408,51 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
         put_x(img[0], 0, CW);
         if (m0 + BM < m1) request(m0 + BM);
     }
-    for (int64_t m = m0; m < m1; m += BM) {
-        CK_BARRIER();
-        const bool more = m + BM < m1;
-        const ck_u32x4* im = img[turn];
-        ck_u32x4* next = img[turn ^ 1];
-        constexpr int S = BM / 16;
+    // one chunk: S x P x F x F matrix instructions; STAGE: the next chunk's registers are turned and written in between, in
+    // the same run of instructions, so that the vector unit works while the matrix unit does
+    constexpr int S = BM / 16;
+    auto fetch_b = [&](const ck_u32x4* im, int s, ck_bf16x8 (&b)[F]) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int mblk = s * 2 + fh;
-            ck_bf16x8 b[F];
+        for (int j = 0; j < F; ++j) b[j] = __builtin_bit_cast(ck_bf16x8, im[P * PIECES + dw_piece<T>(s * 2 + fh, wk + j * 32 + fr)]);
+    };
+    auto fetch_a = [&](const ck_u32x4* im, int s, int p, ck_bf16x8 (&a)[F]) {
 #pragma unroll
-            for (int j = 0; j < F; ++j) b[j] = __builtin_bit_cast(ck_bf16x8, im[P * PIECES + dw_piece<T>(mblk, wk + j * 32 + fr)]);
+        for (int i = 0; i < F; ++i) a[i] = __builtin_bit_cast(ck_bf16x8, im[p * PIECES + dw_piece<T>(s * 2 + fh, wn + i * 32 + fr)]);
+    };
+    auto multiply = [&](const ck_u32x4* im, ck_u32x4* next, auto stage) {
+        ck_bf16x8 a[2][F], b[2][F];
+        fetch_b(im, 0, b[0]);
+        fetch_a(im, 0, P - 1, a[0]);
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) {                  // small terms first
-                ck_bf16x8 a[F];
-#pragma unroll
-                for (int i = 0; i < F; ++i) a[i] = __builtin_bit_cast(ck_bf16x8, im[p * PIECES + dw_piece<T>(mblk, wn + i * 32 + fr)]);
-#pragma unroll
-                for (int i = 0; i < F; ++i)
-#pragma unroll
-                    for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+        for (int q = 0; q < S * P; ++q) {                       // small terms first
+            const int s = q / P, s1 = (q + 1) / P;
+            if (q + 1 < S * P) {
+                if (s1 != s) fetch_b(im, s1, b[s1 & 1]);
+                fetch_a(im, s1, P - 1 - (q + 1) % P, a[(q + 1) & 1]);
             }
-            if (more) {
-                if (s == 0) count_db();
-                put_y(next, s * CW / S, (s + 1) * CW / S);
-                put_x(next, s * CW / S, (s + 1) * CW / S);
+            if constexpr (decltype(stage)::value) {
+                if (q % P == 0) {
+                    put_y(next, s * CW / S, (s + 1) * CW / S);
+                    put_x(next, s * CW / S, (s + 1) * CW / S);
+                }
             }
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
         }
-        if (more && m + 2 * BM < m1) request(m + 2 * BM);
+    };
+    int64_t m = m0;
+    for (; m + BM < m1; m += BM) {
+        CK_BARRIER();
+        count_db();
+        multiply(img[turn], img[turn ^ 1], dw_flag<true>{});
+        if (m + 2 * BM < m1) request(m + 2 * BM);
         turn ^= 1;
+    }
+    if (m < m1) {
+        CK_BARRIER();
+        multiply(img[turn], nullptr, dw_flag<false>{});
     }
     float* o = out + (int64_t)blockIdx.y * N * K;
 #pragma unroll
