@@ -228,19 +228,18 @@ template <int DT> struct dw_planes { static constexpr int value = DT == EDGEHIP_
 // rows a chunk: two images of (planes + 1) x T x BM x 2 bytes must fit the 160 KB of LDS
 template <int DT, int T> struct dw_rows { static constexpr int value = T == 256 && DT != EDGEHIP_BF16 ? 32 : 64; };
 
-// x = t[0] + t[1] + ... by truncation to 8 significant bits each; the upper halves of two rows' values in one dword.
-// An infinity or NaN stays in the first term (its remainder would be NaN: zero instead); a NaN whose payload lies in
-// the low half is made quiet first, truncation would turn it into an infinity.
+// x = t[0] + t[1] + ... by truncation to 8 significant bits each; the upper halves of two rows' values in one dword.  An
+// infinity leaves a NaN in the second term (as a NaN does, whose payload truncation could lose): with two or three terms
+// whatever is not finite makes the gradients it reaches NaN.
 template <int P>
 __device__ static inline void dw_split(float x0, float x1, unsigned (&o)[P]) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        unsigned u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-        if (p == 0 && P > 1) { u0 = x0 != x0 ? 0x7fc00000u : u0; u1 = x1 != x1 ? 0x7fc00000u : u1; }
+        const unsigned u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
         o[p] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
         if (p + 1 < P) {
-            x0 = (u0 & 0x7f800000u) == 0x7f800000u ? 0.0f : x0 - __uint_as_float(u0 & 0xffff0000u);
-            x1 = (u1 & 0x7f800000u) == 0x7f800000u ? 0.0f : x1 - __uint_as_float(u1 & 0xffff0000u);
+            x0 -= __uint_as_float(u0 & 0xffff0000u);
+            x1 -= __uint_as_float(u1 & 0xffff0000u);
         }
     }
 }
@@ -260,16 +259,6 @@ template <int DT, int CW> struct dw_y {
 #pragma unroll
         for (int i = 0; i < DWORDS; ++i) d[i] = v[i];
     }
-    __device__ inline void load_some(const char* p, int n) {             // n < CW of them, zeros behind
-#pragma unroll
-        for (int i = 0; i < DWORDS; ++i) d[i] = 0u;
-#pragma unroll
-        for (int c = 0; c < CW; ++c) {
-            if (c >= n) continue;
-            if (DT == EDGEHIP_F32) d[c < DWORDS ? c : 0] = reinterpret_cast<const unsigned*>(p)[c];
-            else d[c / 2 < DWORDS ? c / 2 : 0] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[c] << (16 * (c & 1));
-        }
-    }
     __device__ inline float get(int c) const {
         if (DT == EDGEHIP_F32) return __uint_as_float(d[c < DWORDS ? c : 0]);
         const unsigned w = d[c / 2 < DWORDS ? c / 2 : 0];
@@ -283,7 +272,8 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
                                                                 const int8_t* __restrict__ exps, int64_t M, int N, int K, int KG,
                                                                 int64_t rows_per_split, int nt, int kt, float* __restrict__ out,
                                                                 float* __restrict__ db) {
-    constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT, T>::value, CW = T * BM / 2048, W = T / 2, F = W / 32;
+    constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT, T>::value, CW = 4, W = T / 2, F = W / 32;
+    constexpr int MB = 256 / (T / CW), U = BM / 8 / MB;         // m-blocks staged at once, times the U pieces of a thread
     constexpr int PIECES = BM / 8 * T, ES = DT == EDGEHIP_F32 ? 4 : 2;
     __shared__ ck_u32x4 img[2][(P + 1) * PIECES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -293,94 +283,87 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
     const int total = nt * kt;
     if ((total & 7) == 0) id = (id & 7) * (total >> 3) + (id >> 3);
     const int band = id / (4 * kt), left = nt - band * 4 < 4 ? nt - band * 4 : 4, in = id - band * 4 * kt;
-    const int n0 = (band * 4 + in % left) * T, ktile = in / left, k0 = ktile * T;
+    const int ktile = in / left, k0 = ktile * T;
+    // the last n-tile is moved back to end with dY: its first columns are then made twice, to the same bits
+    int n0 = (band * 4 + in % left) * T;
+    if (n0 + T > N) n0 = N > T ? N - T : 0;
     const int64_t m0 = (int64_t)blockIdx.y * rows_per_split;
     const int64_t m1 = m0 + rows_per_split < M ? m0 + rows_per_split : M;
-    // staging: this thread's columns and eight rows of both operands
+    // Staging: four columns and, U times, eight rows of both operands a thread.  No access leaves its row: columns behind the
+    // end of a dY narrower than the tile are those of its last four (written again where they belong), a word of codes that
+    // would pass the end of its row is read further left and shifted.  Rows behind the last one are read from it, with
+    // step 0.
     const int c0 = (tid % (T / CW)) * CW, mb = tid / (T / CW);
-    const char* yp = reinterpret_cast<const char*>(dY) + (m0 + mb * 8) * (int64_t)N * ES + (int64_t)(n0 + c0) * ES;
-    const int8_t* xp = codes + (m0 + mb * 8) * (int64_t)K + k0 + c0;
-    const int8_t* ep = exps + (m0 + mb * 8) * (int64_t)KG + ((k0 + c0) >> 6);
-    const int ny = N - n0 - c0, nx = K - k0 - c0;
-    const bool inner = n0 + T <= N && k0 + T <= K;
-    dw_y<DT, CW> y[8];
-    unsigned x[8][CW / 4];
-    int e[8];
-    auto request = [&](int64_t m) {
-        const int64_t r0 = m + mb * 8;
-        if (inner && m + BM <= m1) {
+    const int yc = c0 + CW <= N - n0 ? c0 : N - n0 - CW;
+    const int kc = k0 + c0 < K ? k0 + c0 : K - 1, kw = kc + CW <= K ? kc : K - CW, xs = (kc - kw) * 8;
+    const unsigned yv = (unsigned)(((int64_t)mb * 8 * N + n0 + yc) * ES), xv = (unsigned)(mb * 8 * K + kw), ev = (unsigned)(mb * 8 * KG + (kc >> 6));
+    dw_y<DT, CW> y[U][8];
+    unsigned x[U][8];
+    int e[U][8];
+    typedef unsigned word __attribute__((aligned(1)));
+    // piece u of the chunk at row m
+    auto request = [&](int64_t m, int u, auto whole) {
+        const int64_t mu = m + u * MB * 8;
+        if constexpr (decltype(whole)::value) {
+            const char* yp = reinterpret_cast<const char*>(dY) + mu * N * ES;
+            const int8_t* xp = codes + mu * K;
+            const int8_t* ep = exps + mu * KG;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                y[i].load(yp + (int64_t)i * N * ES);
-                typedef unsigned vec __attribute__((ext_vector_type(CW / 4), aligned(1)));
-                const vec v = *reinterpret_cast<const vec*>(xp + (int64_t)i * K);
-#pragma unroll
-                for (int j = 0; j < CW / 4; ++j) x[i][j] = v[j];
-                e[i] = ep[(int64_t)i * KG];
+                y[u][i].load(yp + (int64_t)i * N * ES + yv);
+                x[u][i] = *reinterpret_cast<const word*>(xp + (int64_t)i * K + xv);
+                e[u][i] = (ep + (int64_t)i * KG)[ev];
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool live = r0 + i < m1;
-                if (live && ny >= CW) y[i].load(yp + (int64_t)i * N * ES);
-                else y[i].load_some(yp + (int64_t)i * N * ES, live ? ny : 0);
-                e[i] = 0;
-#pragma unroll
-                for (int j = 0; j < CW / 4; ++j) x[i][j] = 0u;
-                if (live && nx > 0) {
-                    e[i] = ep[(int64_t)i * KG];
-#pragma unroll
-                    for (int c = 0; c < CW; ++c)
-                        if (c < nx) x[i][c / 4] |= ((unsigned)xp[(int64_t)i * K + c] & 0xffu) << (8 * (c & 3));
-                }
+                const int64_t r = mu + mb * 8 + i, q = r < m1 ? r : m1 - 1;
+                y[u][i].load(reinterpret_cast<const char*>(dY) + (q * N + n0 + yc) * ES);
+                x[u][i] = *reinterpret_cast<const word*>(codes + q * K + kw);
+                e[u][i] = r < m1 ? exps[q * KG + (kc >> 6)] : -127;
             }
         }
-        yp += (int64_t)BM * N * ES;
-        xp += (int64_t)BM * K;
-        ep += (int64_t)BM * KG;
     };
     float bsum[CW];
 #pragma unroll
     for (int c = 0; c < CW; ++c) bsum[c] = 0.0f;
-    auto put_y = [&](ck_u32x4* im, int ca, int cb) {
+    auto put = [&](ck_u32x4* im, int u) {
+        const int mblk = u * MB + mb;
 #pragma unroll
-        for (int c = ca; c < cb; ++c) {
+        for (int c = 0; c < CW; ++c) {
             ck_u32x4 w[P];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 unsigned o[P];
-                if (DT == EDGEHIP_BF16) o[0] = __builtin_amdgcn_perm(y[2 * i + 1].d[c / 2], y[2 * i].d[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-                else dw_split<P>(y[2 * i].get(c), y[2 * i + 1].get(c), o);
+                if (DT == EDGEHIP_BF16) o[0] = __builtin_amdgcn_perm(y[u][2 * i + 1].d[c / 2], y[u][2 * i].d[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+                else dw_split<P>(y[u][2 * i].get(c), y[u][2 * i + 1].get(c), o);
 #pragma unroll
                 for (int p = 0; p < P; ++p) w[p][i] = o[p];
             }
 #pragma unroll
-            for (int p = 0; p < P; ++p) im[p * PIECES + dw_piece<T>(mb, c0 + c)] = w[p];
+            for (int p = 0; p < P; ++p) im[p * PIECES + dw_piece<T>(mblk, yc + c)] = w[p];
         }
-    };
-    auto put_x = [&](ck_u32x4* im, int ca, int cb) {
         float st[8], off[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             // exponent -128 gives -infinity, and such a group's codes are 0: code * step is NaN, as it should be
-            st[i] = __uint_as_float((unsigned)(127 + e[i]) << 23);
+            st[i] = __uint_as_float((unsigned)(127 + e[u][i]) << 23);
             off[i] = -128.0f * st[i];
+            x[u][i] = (x[u][i] >> xs) ^ 0x80808080u;
         }
 #pragma unroll
-        for (int c = ca; c < cb; ++c) {
+        for (int c = 0; c < CW; ++c) {
             ck_u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float v[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 2; ++h)
                     // code + 128 as an unsigned byte, times the step, minus 128 steps: both exact
-                    const unsigned b = ((x[2 * i + h][c / 4] ^ 0x80808080u) >> (8 * (c & 3))) & 0xffu;
-                    v[h] = __builtin_fmaf((float)b, st[2 * i + h], off[2 * i + h]);
-                }
+                    v[h] = __builtin_fmaf((float)((x[u][2 * i + h] >> (8 * c)) & 0xffu), st[2 * i + h], off[2 * i + h]);
                 w[i] = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
             }
-            im[P * PIECES + dw_piece<T>(mb, c0 + c)] = w;
+            im[P * PIECES + dw_piece<T>(mblk, c0 + c)] = w;
         }
     };
     ck_f32x16 acc[F][F];
@@ -392,21 +375,30 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     const int wn = (wave & 1) * W, wk = (wave >> 1) * W, fr = lane & 31, fh = lane >> 5;
     int turn = 0, chunk = 0;
-    auto count_db = [&]() {
+    // the column sums of the chunk at row m, which the registers hold
+    auto count_db = [&](int64_t m) {
         if (db && chunk % kt == ktile) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int c = 0; c < CW; ++c) bsum[c] += y[i].get(c);
+                for (int i = 0; i < 8; ++i) {
+                    const bool live = m + (u * MB + mb) * 8 + i < m1;
+#pragma unroll
+                    for (int c = 0; c < CW; ++c) bsum[c] += live ? y[u][i].get(c) : 0.0f;
+                }
         }
         ++chunk;
     };
     if (m0 < m1) {
-        request(m0);
-        count_db();
-        put_y(img[0], 0, CW);
-        put_x(img[0], 0, CW);
-        if (m0 + BM < m1) request(m0 + BM);
+#pragma unroll
+        for (int u = 0; u < U; ++u) request(m0, u, dw_flag<false>{});
+        count_db(m0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) put(img[0], u);
+        if (m0 + BM < m1) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) request(m0 + BM, u, dw_flag<false>{});
+        }
     }
     // one chunk: S x P x F x F matrix instructions; STAGE: the next chunk's registers are turned and written in between, in
     // the same run of instructions, so that the vector unit works while the matrix unit does
@@ -419,7 +411,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
 #pragma unroll
         for (int i = 0; i < F; ++i) a[i] = __builtin_bit_cast(ck_bf16x8, im[p * PIECES + dw_piece<T>(s * 2 + fh, wn + i * 32 + fr)]);
     };
-    auto multiply = [&](const ck_u32x4* im, ck_u32x4* next, auto stage) {
+    auto multiply = [&](const ck_u32x4* im, ck_u32x4* next, int64_t after, auto stage, auto whole) {
         ck_bf16x8 a[2][F], b[2][F];
         fetch_b(im, 0, b[0]);
         fetch_a(im, 0, P - 1, a[0]);
@@ -431,28 +423,35 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
                 fetch_a(im, s1, P - 1 - (q + 1) % P, a[(q + 1) & 1]);
             }
             if constexpr (decltype(stage)::value) {
-                if (q % P == 0) {
-                    put_y(next, s * CW / S, (s + 1) * CW / S);
-                    put_x(next, s * CW / S, (s + 1) * CW / S);
-                }
+                if (q % (S * P / U) == 0) put(next, q / (S * P / U));
             }
 #pragma unroll
             for (int i = 0; i < F; ++i)
 #pragma unroll
                 for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
+            if constexpr (decltype(stage)::value) {
+                // the registers just written are free again: they are filled for the chunk after the next, most of a chunk's
+                // time before they are needed
+                if (q % (S * P / U) == 0 && (decltype(whole)::value || after < m1)) request(after, q / (S * P / U), whole);
+            }
         }
     };
     int64_t m = m0;
+    for (; m + 3 * BM <= m1; m += BM) {
+        CK_BARRIER();
+        count_db(m + BM);
+        multiply(img[turn], img[turn ^ 1], m + 2 * BM, dw_flag<true>{}, dw_flag<true>{});
+        turn ^= 1;
+    }
     for (; m + BM < m1; m += BM) {
         CK_BARRIER();
-        count_db();
-        multiply(img[turn], img[turn ^ 1], dw_flag<true>{});
-        if (m + 2 * BM < m1) request(m + 2 * BM);
+        count_db(m + BM);
+        multiply(img[turn], img[turn ^ 1], m + 2 * BM, dw_flag<true>{}, dw_flag<false>{});
         turn ^= 1;
     }
     if (m < m1) {
         CK_BARRIER();
-        multiply(img[turn], nullptr, dw_flag<false>{});
+        multiply(img[turn], nullptr, m1, dw_flag<false>{}, dw_flag<false>{});
     }
     float* o = out + (int64_t)blockIdx.y * N * K;
 #pragma unroll
@@ -465,19 +464,40 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
                 if (n < N && k < K) o[(int64_t)n * K + k] = acc[i][j][r];
             }
     if (db) {
-        // the BM / 8 threads that hold one column's sums, through LDS
+        // the MB threads that hold one column's sums, through LDS
         __syncthreads();
         float* red = reinterpret_cast<float*>(img[0]);
 #pragma unroll
-        for (int c = 0; c < CW; ++c) red[mb * T + c0 + c] = bsum[c];
+        for (int c = 0; c < CW; ++c) red[mb * T + yc + c] = bsum[c];
         __syncthreads();
         if (tid < T && n0 + tid < N) {
             float s = 0.0f;
 #pragma unroll
-            for (int b = 0; b < BM / 8; ++b) s += red[b * T + tid];
+            for (int b = 0; b < MB; ++b) s += red[b * T + tid];
             db[((int64_t)blockIdx.y * kt + ktile) * N + n0 + tid] = s;
         }
     }
+}
+
+// Fewer than four columns on one side: nothing for a tile.  A thread owns one value of dW, 256 of them a block; rows as
+// above.  HBM bound (the wide side is read once, by neighbouring threads).
+template <int DT>
+__global__ __launch_bounds__(256) void k_ck_dw_thin(const void* __restrict__ dY, const int8_t* __restrict__ codes, const int8_t* __restrict__ exps,
+                                                    int64_t M, int N, int K, int KG, int64_t rows_per_split, float* __restrict__ out,
+                                                    float* __restrict__ db) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)N * K) return;
+    const int n = (int)(i / K), k = (int)(i % K);
+    const int64_t m0 = (int64_t)blockIdx.y * rows_per_split, m1 = m0 + rows_per_split < M ? m0 + rows_per_split : M;
+    float a = 0.0f, b = 0.0f;
+#pragma unroll 4
+    for (int64_t m = m0; m < m1; ++m) {
+        const float y = (float)reinterpret_cast<const typename eh_elem<DT>::type*>(dY)[m * N + n];
+        a = __builtin_fmaf(y, (float)codes[m * K + k] * ck_step(exps[m * KG + (k >> 6)]), a);
+        b += y;
+    }
+    out[(int64_t)blockIdx.y * N * K + i] = a;
+    if (db && k == 0) db[(int64_t)blockIdx.y * N + n] = b;
 }
 
 // Sums of the partial results, in order: 64 columns of four x 16 strips of partials a block; the strips meet in LDS.  The
@@ -523,6 +543,11 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
     p.tile = N > 128 && K > 128 ? 256 : 128;
     p.nt = eh_cdiv(N, p.tile);
     p.kt = eh_cdiv(K, p.tile);
+    if (N < 4 || K < 4) {                        // k_ck_dw_thin: blocks of 256 values
+        p.tile = 0;
+        p.nt = eh_cdiv((int64_t)N * K, 256);
+        p.kt = 1;
+    }
     const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 255) / 256;
     int64_t s = tiles >= 256 ? 1 : 256 / tiles;
     if (s > most) s = most;
@@ -536,7 +561,7 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
 
 static int dw_check(int32_t dtype, int64_t M, int32_t N, int32_t K) {
     EH_CHECK_ARG(eh_dtype_ok(dtype) && M >= 0 && N >= 1 && K >= 1);
-    if (N > (1 << 22) || K > (1 << 22)) return EDGEHIP_ERR_TOO_LARGE;        // 32-bit column arithmetic
+    if (N > (1 << 22) || K > (1 << 22)) return EDGEHIP_ERR_TOO_LARGE;        // offsets within 64 rows are 32 bits
     return EDGEHIP_OK;
 }
 
@@ -569,11 +594,13 @@ extern "C" int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const i
     const dim3 grid(p.nt * p.kt, p.splits), block(256);
     const int KG = (K + CK_GROUP - 1) / CK_GROUP;
 #define DW_GO(DT, T) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw<DT, T>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, p.nt, p.kt, part, pdb))
-#define DW_TILE(DT) do { if (p.tile == 256) DW_GO(DT, 256); else DW_GO(DT, 128); } while (0)
+#define DW_THIN(DT) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw_thin<DT>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, part, pdb))
+#define DW_TILE(DT) do { if (p.tile == 256) DW_GO(DT, 256); else if (p.tile) DW_GO(DT, 128); else DW_THIN(DT); } while (0)
     if (dtype == EDGEHIP_F32) DW_TILE(EDGEHIP_F32);
     else if (dtype == EDGEHIP_BF16) DW_TILE(EDGEHIP_BF16);
     else DW_TILE(EDGEHIP_F16);
 #undef DW_TILE
+#undef DW_THIN
 #undef DW_GO
     EH_LAUNCH_CHECK();
     const int64_t n = (int64_t)N * K;
