@@ -225,8 +225,8 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 #define CK_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
 template <int DT> struct dw_planes { static constexpr int value = DT == EDGEHIP_BF16 ? 1 : DT == EDGEHIP_F16 ? 2 : 3; };
-// rows a chunk: two images of (planes + 1) x T x BM x 2 bytes must fit the 160 KB of LDS
-template <int DT, int T> struct dw_rows { static constexpr int value = T == 256 && DT != EDGEHIP_BF16 ? 32 : 64; };
+// rows a chunk: two images of (planes + 1) x T x BM x 2 bytes must fit the 160 KB of LDS, twice for two blocks a CU (T = 128)
+template <int DT> struct dw_rows { static constexpr int value = DT == EDGEHIP_BF16 ? 64 : 32; };
 
 // x = t[0] + t[1] + ... by truncation to 8 significant bits each; the upper halves of two rows' values in one dword.  An
 // infinity leaves a NaN in the second term (as a NaN does, whose payload truncation could lose): with two or three terms
@@ -244,18 +244,29 @@ __device__ static inline void dw_split(float x0, float x1, unsigned (&o)[P]) {
     }
 }
 
+template <int CW> struct dw_word { typedef unsigned type __attribute__((aligned(1))); };
+template <> struct dw_word<2> { typedef unsigned short type __attribute__((aligned(1))); };
 template <bool B> struct dw_flag { static constexpr bool value = B; };
 
 template <int T>
 __device__ static inline int dw_piece(int mblk, int c) { return mblk * T + ((c & ~7) | ((c ^ (c >> 3)) & 7)); }
 
+// a global address whose base is in scalar registers
+#define DW_GLOBAL __attribute__((address_space(1)))
+typedef const DW_GLOBAL char* dw_addr;
+__device__ static inline dw_addr dw_uniform(const void* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(v >> 32));
+    return reinterpret_cast<dw_addr>(((uint64_t)hi << 32) | lo);
+}
+
 // CW consecutive values of a dY row as they stand in memory: DWORDS registers
 template <int DT, int CW> struct dw_y {
     static constexpr int DWORDS = CW * (DT == EDGEHIP_F32 ? 4 : 2) / 4;
     unsigned d[DWORDS];
-    __device__ inline void load(const char* p) {
+    __device__ inline void load(dw_addr p) {
         typedef unsigned vec __attribute__((ext_vector_type(DWORDS), aligned(2)));
-        const vec v = *reinterpret_cast<const vec*>(p);
+        const vec v = *reinterpret_cast<const DW_GLOBAL vec*>(p);
 #pragma unroll
         for (int i = 0; i < DWORDS; ++i) d[i] = v[i];
     }
@@ -268,11 +279,11 @@ template <int DT, int CW> struct dw_y {
 };
 
 template <int DT, int T>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __restrict__ dY, const int8_t* __restrict__ codes,
+__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __restrict__ dY, const int8_t* __restrict__ codes,
                                                                 const int8_t* __restrict__ exps, int64_t M, int N, int K, int KG,
                                                                 int64_t rows_per_split, int nt, int kt, float* __restrict__ out,
                                                                 float* __restrict__ db) {
-    constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT, T>::value, CW = 4, W = T / 2, F = W / 32;
+    constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT>::value, CW = T * BM >= 8192 ? 4 : 2, W = T / 2, F = W / 32;
     constexpr int MB = 256 / (T / CW), U = BM / 8 / MB;         // m-blocks staged at once, times the U pieces of a thread
     constexpr int PIECES = BM / 8 * T, ES = DT == EDGEHIP_F32 ? 4 : 2;
     __shared__ ck_u32x4 img[2][(P + 1) * PIECES];
@@ -289,37 +300,39 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
     if (n0 + T > N) n0 = N > T ? N - T : 0;
     const int64_t m0 = (int64_t)blockIdx.y * rows_per_split;
     const int64_t m1 = m0 + rows_per_split < M ? m0 + rows_per_split : M;
-    // Staging: four columns and, U times, eight rows of both operands a thread.  No access leaves its row: columns behind the
-    // end of a dY narrower than the tile are those of its last four (written again where they belong), a word of codes that
-    // would pass the end of its row is read further left and shifted.  Rows behind the last one are read from it, with
-    // step 0.
+    // Staging: CW (2 or 4) columns and, U times, eight rows of both operands a thread.  No access leaves its tensor: columns behind
+    // the end of a dY narrower than the tile are those of its last CW (written again where they belong), a word of codes
+    // that passes the end of its row reads into the next one (columns behind the end go nowhere), in the last chunk it is
+    // read further left and shifted.  Rows behind the last one are read from it, with step 0.
     const int c0 = (tid % (T / CW)) * CW, mb = tid / (T / CW);
     const int yc = c0 + CW <= N - n0 ? c0 : N - n0 - CW;
     const int kc = k0 + c0 < K ? k0 + c0 : K - 1, kw = kc + CW <= K ? kc : K - CW, xs = (kc - kw) * 8;
-    const unsigned yv = (unsigned)(((int64_t)mb * 8 * N + n0 + yc) * ES), xv = (unsigned)(mb * 8 * K + kw), ev = (unsigned)(mb * 8 * KG + (kc >> 6));
+    const unsigned yv = (unsigned)(((int64_t)mb * 8 * N + n0 + yc) * ES), xv = (unsigned)(mb * 8 * K + kc), ev = (unsigned)(mb * 8 * KG + (kc >> 6));
     dw_y<DT, CW> y[U][8];
     unsigned x[U][8];
     int e[U][8];
-    typedef unsigned word __attribute__((aligned(1)));
+    typedef typename dw_word<CW>::type word;
     // piece u of the chunk at row m
     auto request = [&](int64_t m, int u, auto whole) {
         const int64_t mu = m + u * MB * 8;
         if constexpr (decltype(whole)::value) {
-            const char* yp = reinterpret_cast<const char*>(dY) + mu * N * ES;
-            const int8_t* xp = codes + mu * K;
-            const int8_t* ep = exps + mu * KG;
+            // (bases of the scalar unit, one 32-bit offset a lane: no address arithmetic in the vector unit)
+            const dw_addr yp = dw_uniform(reinterpret_cast<const char*>(dY) + mu * N * ES), xp = dw_uniform(codes + mu * K),
+                          ep = dw_uniform(exps + mu * KG);
+            unsigned yo = yv, xo = xv, eo = ev;
+            asm("" : "+v"(yo), "+v"(xo), "+v"(eo));             // extended to 64 bits here, where the load can fold it
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                y[u][i].load(yp + (int64_t)i * N * ES + yv);
-                x[u][i] = *reinterpret_cast<const word*>(xp + (int64_t)i * K + xv);
-                e[u][i] = (ep + (int64_t)i * KG)[ev];
+                y[u][i].load(yp + (int64_t)i * N * ES + yo);
+                x[u][i] = *reinterpret_cast<const DW_GLOBAL word*>(xp + (int64_t)i * K + xo);
+                e[u][i] = *reinterpret_cast<const DW_GLOBAL int8_t*>(ep + (int64_t)i * KG + eo);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int64_t r = mu + mb * 8 + i, q = r < m1 ? r : m1 - 1;
-                y[u][i].load(reinterpret_cast<const char*>(dY) + (q * N + n0 + yc) * ES);
-                x[u][i] = *reinterpret_cast<const word*>(codes + q * K + kw);
+                y[u][i].load(reinterpret_cast<dw_addr>(reinterpret_cast<uint64_t>(dY)) + (q * N + n0 + yc) * ES);
+                x[u][i] = (unsigned)*reinterpret_cast<const word*>(codes + q * K + kw) >> xs;
                 e[u][i] = r < m1 ? exps[q * KG + (kc >> 6)] : -127;
             }
         }
@@ -343,14 +356,11 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
 #pragma unroll
             for (int p = 0; p < P; ++p) im[p * PIECES + dw_piece<T>(mblk, yc + c)] = w[p];
         }
-        float st[8], off[8];
+        float st[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i)
             // exponent -128 gives -infinity, and such a group's codes are 0: code * step is NaN, as it should be
             st[i] = __uint_as_float((unsigned)(127 + e[u][i]) << 23);
-            off[i] = -128.0f * st[i];
-            x[u][i] = (x[u][i] >> xs) ^ 0x80808080u;
-        }
 #pragma unroll
         for (int c = 0; c < CW; ++c) {
             ck_u32x4 w;
@@ -358,9 +368,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
             for (int i = 0; i < 4; ++i) {
                 float v[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    // code + 128 as an unsigned byte, times the step, minus 128 steps: both exact
-                    v[h] = __builtin_fmaf((float)((x[u][2 * i + h] >> (8 * c)) & 0xffu), st[2 * i + h], off[2 * i + h]);
+                for (int h = 0; h < 2; ++h) v[h] = (float)(int8_t)(x[u][2 * i + h] >> (8 * c)) * st[2 * i + h];
                 w[i] = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
             }
             im[P * PIECES + dw_piece<T>(mblk, c0 + c)] = w;
@@ -437,7 +445,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 1) void k_ck_dw(const void* __r
         }
     };
     int64_t m = m0;
-    for (; m + 3 * BM <= m1; m += BM) {
+    for (; m + 3 * BM < m1; m += BM) {
         CK_BARRIER();
         count_db(m + BM);
         multiply(img[turn], img[turn ^ 1], m + 2 * BM, dw_flag<true>{}, dw_flag<true>{});
@@ -537,7 +545,7 @@ __global__ __launch_bounds__(1024) void k_ck_dw_sum(const float* __restrict__ pa
 }
 
 struct dw_plan { int tile, nt, kt, splits; int64_t rows; };
-// The tile and the splits of the rows: one block a CU fills the chip, a split has at least 256 rows
+// The tile and the splits of the rows: the chip holds one block of the larger tile a CU, two of the smaller
 static dw_plan dw_choose(int64_t M, int N, int K) {
     dw_plan p;
     p.tile = N > 128 && K > 128 ? 256 : 128;
@@ -549,7 +557,8 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
         p.kt = 1;
     }
     const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 255) / 256;
-    int64_t s = tiles >= 256 ? 1 : 256 / tiles;
+    const int64_t room = p.tile == 256 ? 256 : 512;      // blocks the chip holds at once
+    int64_t s = tiles >= room ? 1 : room / tiles;
     if (s > most) s = most;
     if (s < 1) s = 1;
     p.rows = ((M + s - 1) / s + 63) / 64 * 64;
