@@ -285,6 +285,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
                                                                 float* __restrict__ db) {
     constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT>::value, CW = T * BM >= 8192 ? 4 : 2, W = T / 2, F = W / 32;
     constexpr int MB = 256 / (T / CW), U = BM / 8 / MB;         // m-blocks staged at once, times the U pieces of a thread
+    constexpr int D = T == 256 ? 1 : 2;                          // chunks requested ahead of the one being staged
     constexpr int PIECES = BM / 8 * T, ES = DT == EDGEHIP_F32 ? 4 : 2;
     __shared__ ck_u32x4 img[2][(P + 1) * PIECES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -308,13 +309,13 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
     const int yc = c0 + CW <= N - n0 ? c0 : N - n0 - CW;
     const int kc = k0 + c0 < K ? k0 + c0 : K - 1, kw = kc + CW <= K ? kc : K - CW, xs = (kc - kw) * 8;
     const unsigned yv = (unsigned)(((int64_t)mb * 8 * N + n0 + yc) * ES), xv = (unsigned)(mb * 8 * K + kc), ev = (unsigned)(mb * 8 * KG + (kc >> 6));
-    dw_y<DT, CW> y[U][8];
-    unsigned x[U][8];
-    int e[U][8];
+    dw_y<DT, CW> y[D * U][8];
+    unsigned x[D * U][8];
+    int e[D * U][8];
     typedef typename dw_word<CW>::type word;
-    // piece u of the chunk at row m
+    // piece u (of register set u / U) of the chunk at row m
     auto request = [&](int64_t m, int u, auto whole) {
-        const int64_t mu = m + u * MB * 8;
+        const int64_t mu = m + u % U * MB * 8;
         if constexpr (decltype(whole)::value) {
             // (bases of the scalar unit, one 32-bit offset a lane: no address arithmetic in the vector unit)
             const dw_addr yp = dw_uniform(reinterpret_cast<const char*>(dY) + mu * N * ES), xp = dw_uniform(codes + mu * K),
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
 #pragma unroll
     for (int c = 0; c < CW; ++c) bsum[c] = 0.0f;
     auto put = [&](ck_u32x4* im, int u) {
-        const int mblk = u * MB + mb;
+        const int mblk = u % U * MB + mb;
 #pragma unroll
         for (int c = 0; c < CW; ++c) {
             ck_u32x4 w[P];
@@ -383,8 +384,8 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     const int wn = (wave & 1) * W, wk = (wave >> 1) * W, fr = lane & 31, fh = lane >> 5;
     int turn = 0, chunk = 0;
-    // the column sums of the chunk at row m, which the registers hold
-    auto count_db = [&](int64_t m) {
+    // the column sums of the chunk at row m, which register set `set` holds
+    auto count_db = [&](int64_t m, int set) {
         if (db && chunk % kt == ktile) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -392,20 +393,21 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
                 for (int i = 0; i < 8; ++i) {
                     const bool live = m + (u * MB + mb) * 8 + i < m1;
 #pragma unroll
-                    for (int c = 0; c < CW; ++c) bsum[c] += live ? y[u][i].get(c) : 0.0f;
+                    for (int c = 0; c < CW; ++c) bsum[c] += live ? y[set * U + u][i].get(c) : 0.0f;
                 }
         }
         ++chunk;
     };
     if (m0 < m1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) request(m0, u, dw_flag<false>{});
-        count_db(m0);
+        for (int u = 0; u < D * U; ++u)
+            if (m0 + u / U * BM < m1) request(m0 + u / U * BM, u, dw_flag<false>{});
+        count_db(m0, 0);
 #pragma unroll
         for (int u = 0; u < U; ++u) put(img[0], u);
-        if (m0 + BM < m1) {
+        if (m0 + D * BM < m1) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) request(m0 + BM, u, dw_flag<false>{});
+            for (int u = 0; u < U; ++u) request(m0 + D * BM, u, dw_flag<false>{});
         }
     }
     // one chunk: S x P x F x F matrix instructions; STAGE: the next chunk's registers are turned and written in between, in
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
 #pragma unroll
         for (int i = 0; i < F; ++i) a[i] = __builtin_bit_cast(ck_bf16x8, im[p * PIECES + dw_piece<T>(s * 2 + fh, wn + i * 32 + fr)]);
     };
-    auto multiply = [&](const ck_u32x4* im, ck_u32x4* next, int64_t after, auto stage, auto whole) {
+    auto multiply = [&](const ck_u32x4* im, ck_u32x4* next, int64_t after, int set, auto stage, auto whole) {
         ck_bf16x8 a[2][F], b[2][F];
         fetch_b(im, 0, b[0]);
         fetch_a(im, 0, P - 1, a[0]);
@@ -431,35 +433,44 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
                 fetch_a(im, s1, P - 1 - (q + 1) % P, a[(q + 1) & 1]);
             }
             if constexpr (decltype(stage)::value) {
-                if (q % (S * P / U) == 0) put(next, q / (S * P / U));
+                if (q % (S * P / U) == 0) put(next, set * U + q / (S * P / U));
             }
 #pragma unroll
             for (int i = 0; i < F; ++i)
 #pragma unroll
                 for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[q & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
             if constexpr (decltype(stage)::value) {
-                // the registers just written are free again: they are filled for the chunk after the next, most of a chunk's
-                // time before they are needed
-                if (q % (S * P / U) == 0 && (decltype(whole)::value || after < m1)) request(after, q / (S * P / U), whole);
+                // the registers just written are free again: they are filled for the chunk D behind the one they held, most of D
+                // chunks' time before they are needed
+                if (q % (S * P / U) == 0 && (decltype(whole)::value || after < m1)) request(after, set * U + q / (S * P / U), whole);
             }
         }
     };
     int64_t m = m0;
-    for (; m + 3 * BM < m1; m += BM) {
-        CK_BARRIER();
-        count_db(m + BM);
-        multiply(img[turn], img[turn ^ 1], m + 2 * BM, dw_flag<true>{}, dw_flag<true>{});
-        turn ^= 1;
+    while (m + (2 * D + 1) * BM < m1) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            CK_BARRIER();
+            count_db(m + BM, (d + 1) % D);
+            multiply(img[turn], img[turn ^ 1], m + (D + 1) * BM, (d + 1) % D, dw_flag<true>{}, dw_flag<true>{});
+            turn ^= 1;
+            m += BM;
+        }
     }
-    for (; m + BM < m1; m += BM) {
-        CK_BARRIER();
-        count_db(m + BM);
-        multiply(img[turn], img[turn ^ 1], m + 2 * BM, dw_flag<true>{}, dw_flag<false>{});
-        turn ^= 1;
+    while (m + BM < m1) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (m + BM >= m1) break;
+            CK_BARRIER();
+            count_db(m + BM, (d + 1) % D);
+            multiply(img[turn], img[turn ^ 1], m + (D + 1) * BM, (d + 1) % D, dw_flag<true>{}, dw_flag<false>{});
+            turn ^= 1;
+            m += BM;
+        }
     }
     if (m < m1) {
         CK_BARRIER();
-        multiply(img[turn], nullptr, m1, dw_flag<false>{}, dw_flag<false>{});
+        multiply(img[turn], nullptr, m1, 0, dw_flag<false>{}, dw_flag<false>{});
     }
     float* o = out + (int64_t)blockIdx.y * N * K;
 #pragma unroll
