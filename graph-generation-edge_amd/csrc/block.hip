@@ -25,6 +25,9 @@
 #include "vec.h"
 
 #define GN_MAX_DIM 8192
+#ifndef GN_FWD_ROUNDS
+#define GN_FWD_ROUNDS 4
+#endif
 
 struct gn_args {
     const void *h, *z, *dho, *dy;
@@ -42,32 +45,49 @@ struct gn_args {
     int want_pre, want_post, want_gate;
 };
 
-// sum over the TPR threads of a row; NW waves per row meet in LDS, two buffers in turn (a wave can only write the
-// buffer of reduction k + 2 after every wave has passed the barrier of k + 1, that is after it has read that of k)
+// TPR threads a row: 8, 16, 32 or 64 (several rows a block of 256), or GN_ROW: the whole block, whole waves of it, as many
+// as the row has pieces of 512 columns.
+#define GN_ROW 1024
+#define GN_WIDE 512                      // blocks up to this size have their own kernels: twice the registers a thread
+#define GN_THREADS(TPR) ((TPR) <= 64 ? 256 : (TPR))
+
+template <int CTRL> __device__ static inline float gn_add_dpp(float v) {
+    return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+// sum over the threads of a row, in every one of them.  Within 16 lanes by lane exchanges of the vector unit (pairs, quads,
+// mirrored halves); the four sums of 16 by the scalar unit's reads.  The waves of a row meet in LDS, two buffers in turn (a
+// wave can only write the buffer of sum k + 2 after every wave has passed the barrier of k + 1, that is after it has read
+// that of k); the barrier waits for LDS only: the next row's requests stay in flight.
 template <int TPR, int NV>
 __device__ static inline void gn_row_sum(float (&v)[NV], float* lds, int& turn) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
+    for (int i = 0; i < NV; ++i) {
+        v[i] = gn_add_dpp<0xB1>(v[i]);                           // quad_perm [1,0,3,2]
+        v[i] = gn_add_dpp<0x4E>(v[i]);                           // quad_perm [2,3,0,1]
+        v[i] = gn_add_dpp<0x141>(v[i]);                          // row_half_mirror
+        if (TPR >= 16) v[i] = gn_add_dpp<0x140>(v[i]);           // row_mirror
+        if (TPR == 32) v[i] += __shfl_xor(v[i], 16, 64);
+        if (TPR >= 64) {
+            const int b = (int)__float_as_uint(v[i]);
+            const float s0 = __uint_as_float((unsigned)__builtin_amdgcn_readlane(b, 0)), s1 = __uint_as_float((unsigned)__builtin_amdgcn_readlane(b, 16));
+            const float s2 = __uint_as_float((unsigned)__builtin_amdgcn_readlane(b, 32)), s3 = __uint_as_float((unsigned)__builtin_amdgcn_readlane(b, 48));
+            v[i] = (s0 + s1) + (s2 + s3);
+        }
     }
     if (TPR > 64) {
-        constexpr int NW = TPR / 64;
+        const int waves = blockDim.x >> 6;
         float* b = lds + turn * 32;
         turn ^= 1;
-        const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) b[wave * 2 + i] = v[i];
+            for (int i = 0; i < NV; ++i) b[(threadIdx.x >> 6) * 2 + i] = v[i];
         }
-        __syncthreads();
-        const int w0 = wave & ~(NW - 1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float s = 0.0f;
+        for (int i = 0; i < NV; ++i) v[i] = 0.0f;
+        for (int w = 0; w < waves; ++w) {
 #pragma unroll
-            for (int w = 0; w < NW; ++w) s += b[(w0 + w) * 2 + i];
-            v[i] = s;
+            for (int i = 0; i < NV; ++i) v[i] += b[w * 2 + i];
         }
     }
 }
@@ -103,14 +123,40 @@ __device__ static inline void gn_stats(const float (&x)[8], int n, float inv_d, 
     r = 1.0f / sqrtf(s[0] * inv_d + eps);
 }
 
-#define GN_BLOCK(TPR) ((TPR) < 256 ? 256 : (TPR))
+// the gate of a row
+template <int DZ, bool TINY>
+__device__ static inline void gn_row_gate(const gn_args& A, const eh_at& at, float (&g)[8]) {
+    if constexpr (DZ == EDGEHIP_F32) {
+        eh_raw8<EDGEHIP_F32> r;
+        eh_get<EDGEHIP_F32, TINY>(r, A.gate, at);
+        r.get(g);
+    } else {
+        eh_raw8<EDGEHIP_F32> r;
+        eh_raw8<DZ> q;
+        float o[8];
+        const bool wide = A.gdt == EDGEHIP_F32;
+        if (wide) eh_get<EDGEHIP_F32, TINY>(r, A.gate, at);
+        else eh_get<DZ, TINY>(q, A.gate, at);
+        r.get(g);
+        q.get(o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = wide ? +g[i] : +o[i];
+    }
+    eh_own<TINY>(g, at.n, at.back);
+}
 
-template <int DH, int DZ, bool LAYER, int TPR>
-__global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_fwd(gn_args A) {
-    constexpr int RPB = GN_BLOCK(TPR) / TPR;
+// what a thread slot reads of its row
+template <int DH, int DZ> struct gn_in {
+    eh_raw8<DZ> z;
+    eh_raw8<DH> h;
+};
+
+template <int DH, int DZ, bool LAYER, int TPR, bool TINY = false>
+__global__ __launch_bounds__(GN_THREADS(TPR)) void k_gn_fwd(gn_args A) {
+    constexpr int RPB = TPR <= 64 ? 256 / TPR : 1;
     __shared__ float lds[64];
     int turn = 0;
-    const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, col = t * 8, n = A.D - col;
+    const int slot = TPR <= 64 ? threadIdx.x / TPR : 0, t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, col = t * 8, n = A.D - col;
     float wpre[8], wpost[8], bpre[8], bpost[8], g[8];
     const int np = n < 0 ? 0 : n;
     eh_load8_any(A.w_pre, A.wdt, col, A.w_pre ? np : 0, wpre, 1.0f);
@@ -120,20 +166,28 @@ __global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_fwd(gn_args A) {
         eh_load8_any(A.b_post, A.wdt, col, A.b_post ? np : 0, bpost, 0.0f);
     }
     eh_load8_any(A.gate, A.gdt, col, A.gkind == EDGEHIP_GATE_VECTOR ? np : 0, g, 1.0f);
-    const int64_t r0 = (int64_t)blockIdx.x * A.rows_per_block;
+    const int64_t end = A.rows * A.D, r0 = (int64_t)blockIdx.x * A.rows_per_block;
     const int64_t r1 = r0 + A.rows_per_block < A.rows ? r0 + A.rows_per_block : A.rows;
     int grp = A.gkind == EDGEHIP_GATE_GROUP ? gn_group_of(A.row_ptr, A.groups, r0) : 0, held = -1;
+    auto request = [&](gn_in<DH, DZ>& in, int64_t row) {
+        const eh_at at = eh_place(row * A.D + col, row < r1 ? n : 0, end);
+        eh_get<DZ, TINY>(in.z, A.z, at);
+        eh_get<DH, TINY>(in.h, A.h, at);
+    };
+    gn_in<DH, DZ> next;
+    request(next, r0 + slot);
     for (int64_t base = r0; base < r1; base += RPB) {
         const int64_t row = base + slot;
         const bool live = row < r1;
-        const int nr = live ? n : 0;
+        const eh_at at = eh_place(row * A.D + col, live ? n : 0, end);
         float z[8], h[8];
-        eh_load8<DZ>(A.z, row * A.D + col, nr, z);
-        eh_load8<DH>(A.h, row * A.D + col, nr, h);
-        if (A.gkind == EDGEHIP_GATE_ROW) {
-            if (A.gdt == EDGEHIP_F32) eh_load8<EDGEHIP_F32>(A.gate, row * A.D + col, nr, g);
-            else eh_load8<DZ>(A.gate, row * A.D + col, nr, g);
-        } else if (A.gkind == EDGEHIP_GATE_GROUP && live) {
+        if (A.gkind == EDGEHIP_GATE_ROW) gn_row_gate<DZ, TINY>(A, at, g);
+        next.z.get(z);
+        next.h.get(h);
+        eh_own<TINY>(z, at.n, at.back);
+        eh_own<TINY>(h, at.n, at.back);
+        request(next, row + RPB);                                // a row ahead
+        if (A.gkind == EDGEHIP_GATE_GROUP && live) {
             while (grp < A.groups && (int64_t)A.row_ptr[grp + 1] <= row) ++grp;
             if (grp != held) {
                 held = grp;
@@ -172,7 +226,7 @@ __global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_fwd(gn_args A) {
 // column sums of the block's row slots -> one partial row
 template <int TPR>
 __device__ static inline void gn_flush(float (&acc)[8], float* lds, float* dst, int D, int slot, int t) {
-    constexpr int RPB = GN_BLOCK(TPR) / TPR;
+    constexpr int RPB = TPR <= 64 ? 256 / TPR : 1;
     const int col = t * 8;
     if (RPB > 1) {
         // slots in turn through LDS: [RPB][TPR * 8] floats, 8 KiB
@@ -180,7 +234,7 @@ __device__ static inline void gn_flush(float (&acc)[8], float* lds, float* dst, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) lds[(slot * 8 + i) * TPR + t] = acc[i];
         __syncthreads();
-        for (int c = threadIdx.x; c < TPR * 8; c += GN_BLOCK(TPR)) {
+        for (int c = threadIdx.x; c < TPR * 8; c += 256) {
             const int i = c / TPR, tt = c % TPR;
             float s = 0.0f;
 #pragma unroll 8
@@ -194,25 +248,78 @@ __device__ static inline void gn_flush(float (&acc)[8], float* lds, float* dst, 
     for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
 }
 
-template <int DH, int DZ, bool LAYER, int TPR>
-__global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_bwd(gn_args A) {
-    constexpr int RPB = GN_BLOCK(TPR) / TPR;
+// The backward kernel needs the norms' weights three times a row; in registers they (and b_post) would cost 24 a thread
+// and with them half of the waves a CU holds.  They stand in LDS instead, as fp32: [vector][half of a thread's
+// eight][thread][4].
+template <int TPR>
+__device__ static inline void gn_par_put(float* par, int t, const float (&v)[8]) {
+    const int T = TPR <= 64 ? TPR : blockDim.x;
+    *reinterpret_cast<float4*>(par + t * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(par + (T + t) * 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <int TPR>
+__device__ static inline void gn_par_get(const float* par, int vec, int t, float (&v)[8]) {
+    const int T = TPR <= 64 ? TPR : blockDim.x;
+    const float4 a = *reinterpret_cast<const float4*>(par + (vec * 2 * T + t) * 4), b = *reinterpret_cast<const float4*>(par + ((vec * 2 + 1) * T + t) * 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+template <int DH, int DZ> struct gn_grad {
+    eh_raw8<DZ> z, dy;
+    eh_raw8<DH> h, d;
+    float4 st;
+};
+
+// waves a SIMD: four (128 registers) with a 16-bit stream, three with fp32 (blocks of 1024 threads: four)
+#define GN_BWD_WAVES(DH) ((DH) == EDGEHIP_F32 ? 3 : 4)
+template <int DH, int DZ, bool LAYER, int TPR, bool TINY = false>
+__global__ __launch_bounds__(GN_THREADS(TPR), (TPR == GN_ROW ? 4 : GN_BWD_WAVES(DH))) void k_gn_bwd(gn_args A) {
+    constexpr int RPB = TPR <= 64 ? 256 / TPR : 1;
+    constexpr bool AHEAD = DH != EDGEHIP_F32;                    // a row's requests a row ahead, where they fit the registers
+    extern __shared__ float par[];
     __shared__ float lds[64];
-    __shared__ float fl[RPB > 1 ? GN_BLOCK(TPR) * 8 : 1];
+    __shared__ float fl[RPB > 1 ? 256 * 8 : 1];
     int turn = 0;
-    const int slot = threadIdx.x / TPR, t = threadIdx.x % TPR, col = t * 8, n = A.D - col;
+    const int slot = TPR <= 64 ? threadIdx.x / TPR : 0, t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, col = t * 8, n = A.D - col;
+    // (gradients that are not given: any tensor of their shape, cleared when it is taken)
+    const void* const dho = A.dho ? A.dho : A.h;
+    const void* const dyp = A.dy ? A.dy : A.z;
+    const bool has_dy = A.dy && A.pre;
     const int np = n < 0 ? 0 : n;
-    float wpre[8], wpost[8], bpost[8], g[8];
-    eh_load8_any(A.w_pre, A.wdt, col, A.w_pre ? np : 0, wpre, 1.0f);
-    eh_load8_any(A.w_post, A.wdt, col, A.w_post ? np : 0, wpost, 1.0f);
-    if (LAYER) eh_load8_any(A.b_post, A.wdt, col, A.b_post ? np : 0, bpost, 0.0f);
+    float g[8];
+    if (slot == 0) {
+        const int T = TPR <= 64 ? TPR : blockDim.x;
+        float v[8];
+        eh_load8_any(A.w_pre, A.wdt, col, A.w_pre ? np : 0, v, 1.0f);
+        gn_par_put<TPR>(par, t, v);
+        eh_load8_any(A.w_post, A.wdt, col, A.w_post ? np : 0, v, 1.0f);
+        gn_par_put<TPR>(par + 8 * T, t, v);
+        if (LAYER) {
+            eh_load8_any(A.b_post, A.wdt, col, A.b_post ? np : 0, v, 0.0f);
+            gn_par_put<TPR>(par + 16 * T, t, v);
+        }
+    }
+    __syncthreads();
     eh_load8_any(A.gate, A.gdt, col, A.gkind == EDGEHIP_GATE_VECTOR ? np : 0, g, 1.0f);
     float awpre[8], awpost[8], abpre[8], abpost[8], ag[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) { awpre[i] = awpost[i] = abpre[i] = abpost[i] = ag[i] = 0.0f; }
-    const int64_t r0 = (int64_t)blockIdx.x * A.rows_per_block;
+    const int64_t end = A.rows * A.D, r0 = (int64_t)blockIdx.x * A.rows_per_block;
     const int64_t r1 = r0 + A.rows_per_block < A.rows ? r0 + A.rows_per_block : A.rows;
     int grp = A.gkind == EDGEHIP_GATE_GROUP ? gn_group_of(A.row_ptr, A.groups, r0) : 0;
+    // u = zhat w_post + b_post
+    auto get_u = [&](const float (&z)[8], float (&u)[8]) {
+        if (!A.post) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = z[i];
+            return;
+        }
+        float w[8], b[8];
+        gn_par_get<TPR>(par, 1, t, w);
+        if (LAYER) gn_par_get<TPR>(par, 2, t, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = LAYER ? z[i] * w[i] + b[i] : z[i] * w[i];
+    };
     for (int64_t s0 = r0; s0 < r1;) {
         // rows of one group (all rows where the gate is not per group)
         int64_t s1 = r1;
@@ -221,46 +328,55 @@ __global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_bwd(gn_args A) {
             if (grp < A.groups && (int64_t)A.row_ptr[grp + 1] < r1) s1 = A.row_ptr[grp + 1];
             eh_load8_any(A.gate, A.gdt, (int64_t)grp * A.D + col, grp < A.groups ? np : 0, g, 0.0f);
         }
+        gn_grad<DH, DZ> in;
+        auto request = [&](int64_t row) {
+            const eh_at at = eh_place(row * A.D + col, row < s1 ? n : 0, end);
+            eh_get<DZ, TINY>(in.z, A.z, at);
+            eh_get<DH, TINY>(in.h, A.h, at);
+            eh_get<DH, TINY>(in.d, dho, at);
+            eh_get<DZ, TINY>(in.dy, dyp, at);
+            in.st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (row < s1) in.st = *reinterpret_cast<const float4*>(A.stats_in + row * 4);
+        };
+        if (AHEAD) request(s0 + slot);
         for (int64_t base = s0; base < s1; base += RPB) {
             const int64_t row = base + slot;
             const bool live = row < s1;
-            const int nr = live ? n : 0;
             const int64_t off = row * A.D + col;
-            float z[8], h[8], d[8], dy[8];
-            eh_load8<DZ>(A.z, off, nr, z);
-            eh_load8<DH>(A.h, off, nr, h);
-            eh_load8<DH>(A.dho, off, A.dho ? nr : 0, d);
-            eh_load8<DZ>(A.dy, off, A.dy && A.pre ? nr : 0, dy);
-            if (A.gkind == EDGEHIP_GATE_ROW) {
-                if (A.gdt == EDGEHIP_F32) eh_load8<EDGEHIP_F32>(A.gate, off, nr, g);
-                else eh_load8<DZ>(A.gate, off, nr, g);
-            }
-            float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (live) st = *reinterpret_cast<const float4*>(A.stats_in + row * 4);
-            float u[8];
+            const eh_at at = eh_place(off, live ? n : 0, end);
+            float z[8], h[8], d[8], dy[8], w[8];
+            if (!AHEAD) request(row);
+            if (A.gkind == EDGEHIP_GATE_ROW) gn_row_gate<DZ, TINY>(A, at, g);
+            in.z.get(z);
+            in.h.get(h);
+            in.d.get(d);
+            in.dy.get(dy);
+            eh_own<TINY>(z, at.n, at.back);
+            eh_own<TINY>(h, at.n, at.back);
+            eh_own<TINY>(d, A.dho ? at.n : 0, at.back);
+            eh_own<TINY>(dy, has_dy ? at.n : 0, at.back);
+            const float4 st = in.st;
+            if (AHEAD) request(row + RPB);
             if (A.post) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    z[i] = (z[i] - st.x) * st.y;                     // zhat
-                    u[i] = z[i] * wpost[i];
-                    if (LAYER) u[i] += bpost[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] = z[i];
+                for (int i = 0; i < 8; ++i) z[i] = (z[i] - st.x) * st.y;          // zhat
             }
             if (A.pre) {
+                float u[8];
+                get_u(z, u);
+                gn_par_get<TPR>(par, 0, t, w);
                 float c[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    h[i] = (A.alpha * h[i] + g[i] * u[i] - st.z) * st.w;     // hhat
+                    h[i] = (A.alpha * h[i] + g[i] * u[i] - st.z) * st.w;         // hhat
                     awpre[i] += dy[i] * h[i];
                     if (LAYER) abpre[i] += dy[i];
-                    dy[i] *= wpre[i];
+                    dy[i] *= w[i];
                     c[0] += i < n ? dy[i] * h[i] : 0.0f;
                     if (LAYER) c[1] += dy[i];
                 }
-                gn_row_sum<TPR, 2>(c, lds, turn);
+                gn_row_sum<TPR, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(c), lds, turn);
+                asm volatile("" ::: "memory");                                   // the weights are read again below, not held
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] += st.w * (dy[i] - h[i] * (c[0] * A.inv_d) - (LAYER ? c[1] * A.inv_d : 0.0f));
             }
@@ -268,30 +384,34 @@ __global__ __launch_bounds__(GN_BLOCK(TPR)) void k_gn_bwd(gn_args A) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = A.alpha * d[i];
             if (live) eh_store8<DH>(A.dh, off, n, o);
+            if (A.want_gate) {
+                get_u(z, o);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = live && i < n ? d[i] * u[i] : 0.0f;
-            if (A.gkind == EDGEHIP_GATE_ROW) {
-                if (A.dgate && live) {
-                    if (A.gdt == EDGEHIP_F32) eh_store8<EDGEHIP_F32>(A.dgate, off, n, o);
-                    else eh_store8<DZ>(A.dgate, off, n, o);
+                for (int i = 0; i < 8; ++i) o[i] = live && i < n ? d[i] * o[i] : 0.0f;
+                if (A.gkind == EDGEHIP_GATE_ROW) {
+                    if (live) {
+                        if (DZ == EDGEHIP_F32 || A.gdt == EDGEHIP_F32) eh_store8<EDGEHIP_F32>(A.dgate, off, n, o);
+                        else eh_store8<DZ>(A.dgate, off, n, o);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ag[i] += o[i];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ag[i] += o[i];
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) d[i] = live && i < n ? d[i] * g[i] : 0.0f;      // du
             if (A.post) {
                 float c[2] = {0.0f, 0.0f};
+                gn_par_get<TPR>(par, 1, t, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     awpost[i] += d[i] * z[i];
                     if (LAYER) abpost[i] += d[i];
-                    d[i] *= wpost[i];
+                    d[i] *= w[i];
                     c[0] += d[i] * z[i];
                     if (LAYER) c[1] += d[i];
                 }
-                gn_row_sum<TPR, 2>(c, lds, turn);
+                gn_row_sum<TPR, LAYER ? 2 : 1>(reinterpret_cast<float (&)[LAYER ? 2 : 1]>(c), lds, turn);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - z[i] * (c[0] * A.inv_d) - (LAYER ? c[1] * A.inv_d : 0.0f));
             }
@@ -358,16 +478,22 @@ __global__ __launch_bounds__(1024) void k_gn_reduce(gn_red R) {
     }
 }
 
+// threads of a row (see GN_ROW): 8 columns each
 static int gn_tpr(int D) {
+    if (D > GN_WIDE * 8) return GN_ROW;
+    if (D > 512) return GN_WIDE;
     int t = 8;
     while (t * 8 < D) t *= 2;
     return t;
 }
-// Rows a block owns.  Forward: few, so that small inputs fill the chip.  Backward: the fewer blocks the fewer partials
-// (5 D floats each at most), but 256 CUs need some blocks each.
-static int gn_rows_per_block(int64_t rows, int D, int bwd) {
-    const int tpr = gn_tpr(D), rpb = (tpr < 256 ? 256 : tpr) / tpr;
-    const int64_t target = bwd ? 1024 : 4096;
+static size_t gn_par_bytes(int D, bool layer) { return (size_t)(D <= 512 ? gn_tpr(D) : (D + 511) / 512 * 64) * 8 * sizeof(float) * (layer ? 3 : 2); }
+static int gn_threads(int D) { return D <= 512 ? 256 : (D + 511) / 512 * 64; }
+// Rows a block owns.  Backward: as many blocks as the chip holds at once; more of them only add partials (5 D floats a block
+// at most) and a second, partly filled round.  Forward: FWD_BLOCKS
+static int gn_rows_per_block(int64_t rows, int D, int stream_dtype, int bwd) {
+    const int rpb = D <= 512 ? 256 / gn_tpr(D) : 1, waves = gn_threads(D) / 64;
+    const int simd = D > GN_WIDE * 8 ? 4 : GN_BWD_WAVES(stream_dtype);
+    const int64_t target = (int64_t)256 * (4 * simd / waves) * (bwd ? 1 : GN_FWD_ROUNDS);
     int64_t per = (rows + target - 1) / target;
     per = (per + rpb - 1) / rpb * rpb;
     return (int)(per < rpb ? rpb : per);
@@ -401,12 +527,19 @@ static gn_args gn_fill(const edgehip_gate_norm* G) {
 
 template <int DH, int DZ, bool LAYER>
 static int gn_launch(const gn_args& A, int nblk, bool bwd, hipStream_t s) {
+    const dim3 block(gn_threads(A.D));
+    if (A.rows * A.D < 8) {
+        if (bwd) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_bwd<DH, DZ, LAYER, 8, true>), dim3(nblk), block, gn_par_bytes(A.D, LAYER), s, A));
+        else EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_fwd<DH, DZ, LAYER, 8, true>), dim3(nblk), block, 0, s, A));
+        EH_LAUNCH_CHECK();
+        return EDGEHIP_OK;
+    }
     switch (gn_tpr(A.D)) {
 #define GN_CASE(T) case T: \
-        if (bwd) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_bwd<DH, DZ, LAYER, T>), dim3(nblk), dim3(GN_BLOCK(T)), 0, s, A)); \
-        else EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_fwd<DH, DZ, LAYER, T>), dim3(nblk), dim3(GN_BLOCK(T)), 0, s, A)); \
+        if (bwd) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_bwd<DH, DZ, LAYER, T>), dim3(nblk), block, gn_par_bytes(A.D, LAYER), s, A)); \
+        else EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_gn_fwd<DH, DZ, LAYER, T>), dim3(nblk), block, 0, s, A)); \
         break;
-        GN_CASE(8) GN_CASE(16) GN_CASE(32) GN_CASE(64) GN_CASE(128) GN_CASE(256) GN_CASE(512) GN_CASE(1024)
+        GN_CASE(8) GN_CASE(16) GN_CASE(32) GN_CASE(64) GN_CASE(GN_WIDE) GN_CASE(GN_ROW)
 #undef GN_CASE
         default: return EDGEHIP_ERR_UNSUPPORTED;
     }
@@ -436,11 +569,11 @@ extern "C" int edgehip_gate_norm_fwd(const edgehip_gate_norm* G, const void* h, 
     EH_CHECK_ARG(h && z && h_out && (!G->pre || y) && ((uintptr_t)stats & 15) == 0);
     gn_args A = gn_fill(G);
     A.h = h; A.z = z; A.ho = h_out; A.y = y; A.stats = stats;
-    A.rows_per_block = gn_rows_per_block(G->rows, G->dim, 0);
+    A.rows_per_block = gn_rows_per_block(G->rows, G->dim, G->stream_dtype, 0);
     return gn_dispatch(G, A, eh_cdiv(G->rows, A.rows_per_block), false, eh_stream(stream));
 }
 
-static int gn_blocks(const edgehip_gate_norm* G) { return eh_cdiv(G->rows, gn_rows_per_block(G->rows, G->dim, 1)); }
+static int gn_blocks(const edgehip_gate_norm* G) { return eh_cdiv(G->rows, gn_rows_per_block(G->rows, G->dim, G->stream_dtype, 1)); }
 
 extern "C" size_t edgehip_gate_norm_workspace_bytes(const edgehip_gate_norm* G) {
     if (gn_check(G) != EDGEHIP_OK) return 0;
@@ -466,7 +599,7 @@ extern "C" int edgehip_gate_norm_bwd(const edgehip_gate_norm* G, const void* dh_
     hipStream_t s = eh_stream(stream);
     gn_args A = gn_fill(G);
     A.h = h; A.z = z; A.dho = dh_out; A.dy = dy; A.dh = dh; A.dz = dz; A.dgate = dgate; A.stats_in = stats;
-    A.rows_per_block = gn_rows_per_block(G->rows, G->dim, 1);
+    A.rows_per_block = gn_rows_per_block(G->rows, G->dim, G->stream_dtype, 1);
     A.nblk = gn_blocks(G);
     A.part = reinterpret_cast<float*>(ws);
     A.gpart = A.part + (size_t)5 * A.nblk * A.D;

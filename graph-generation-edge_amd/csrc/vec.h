@@ -14,6 +14,7 @@ template <> struct eh_elem<EDGEHIP_F16> { typedef _Float16 type; };
 typedef float eh_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned int eh_u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int eh_u32x2u __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned int eh_u32x2h __attribute__((ext_vector_type(2), aligned(2)));
 
 static inline int eh_dtype_ok(int dt) { return dt == EDGEHIP_F32 || dt == EDGEHIP_BF16 || dt == EDGEHIP_F16; }
 
@@ -46,6 +47,46 @@ template <> struct eh_raw8<EDGEHIP_F32> {
     }
 };
 
+// Where a thread's eight values of a row are read, without a branch and without looking at them while the request is in
+// flight: a row's last, partial vector is read whole, into the next row; at the very end of the tensor it is read `back`
+// values earlier; a thread without values (n <= 0) reads whatever its clamped place holds.  eh_own puts that right: values
+// are moved down by `back`, what is not the row's own becomes 0.  The tensor has at least eight values (TINY kernels
+// take smaller ones, value by value).
+struct eh_at { int64_t off; int n, back; };
+__device__ static inline eh_at eh_place(int64_t off, int n, int64_t end) {
+    const int64_t o = off + 8 <= end ? off : end - 8;
+    return eh_at{o, n > 8 ? 8 : n, n > 0 ? (int)(off - o) : 0};
+}
+template <int DT, bool TINY>
+__device__ static inline void eh_get(eh_raw8<DT>& r, const void* base, const eh_at& a) {
+    typedef typename eh_elem<DT>::type T;
+    const T* p = reinterpret_cast<const T*>(base);
+    if (!TINY) {
+        r.load(p + a.off);
+    } else {                                                     // (off is below 0 by 8 - end there, back as much larger)
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < a.n ? p[a.off + a.back + i] : (T)0.0f;
+        __builtin_memcpy(&r, v, sizeof(v));
+    }
+}
+template <bool TINY>
+__device__ static inline void eh_own(float (&v)[8], int n, int back) {
+    if (n < 8) {
+        if (!TINY && back) {
+#pragma unroll
+            for (int s = 1; s < 8; s *= 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float here = v[i], there = v[i + s < 8 ? i + s : 7];
+                    v[i] = back & s ? there : here;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.0f;
+    }
+}
+
 // n of eight values (n <= 0: none); the others read as `fill`
 template <int DT>
 __device__ static inline void eh_load8(const void* base, int64_t off, int n, float (&o)[8], float fill = 0.0f) {
@@ -63,6 +104,11 @@ __device__ static inline void eh_load8(const void* base, int64_t off, int n, flo
 
 // one rounding to the type, to nearest even
 template <int DT>
+__device__ static inline unsigned eh_pack2(float a, float b) {
+    typedef typename eh_elem<DT == EDGEHIP_F32 ? EDGEHIP_BF16 : DT>::type T;
+    return (unsigned)__builtin_bit_cast(unsigned short, (T)a) | ((unsigned)__builtin_bit_cast(unsigned short, (T)b) << 16);
+}
+template <int DT>
 __device__ static inline void eh_store8(void* base, int64_t off, int n, const float (&v)[8]) {
     typedef typename eh_elem<DT>::type T;
     T* p = reinterpret_cast<T*>(base) + off;
@@ -71,19 +117,28 @@ __device__ static inline void eh_store8(void* base, int64_t off, int n, const fl
             *reinterpret_cast<eh_f32x4u*>(p) = eh_f32x4u{v[0], v[1], v[2], v[3]};
             *(reinterpret_cast<eh_f32x4u*>(p) + 1) = eh_f32x4u{v[4], v[5], v[6], v[7]};
         } else {
-            eh_u32x4u w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned lo = __builtin_bit_cast(unsigned short, (typename eh_elem<DT == EDGEHIP_F32 ? EDGEHIP_BF16 : DT>::type)v[2 * i]);
-                const unsigned hi = __builtin_bit_cast(unsigned short, (typename eh_elem<DT == EDGEHIP_F32 ? EDGEHIP_BF16 : DT>::type)v[2 * i + 1]);
-                w[i] = lo | (hi << 16);
-            }
-            *reinterpret_cast<eh_u32x4u*>(p) = w;
+            *reinterpret_cast<eh_u32x4u*>(p) = eh_u32x4u{eh_pack2<DT>(v[0], v[1]), eh_pack2<DT>(v[2], v[3]), eh_pack2<DT>(v[4], v[5]), eh_pack2<DT>(v[6], v[7])};
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = (T)v[i];
+    } else if (n > 0) {                                          // in pieces of four, two and one
+        const bool four = n & 4;
+        if (DT == EDGEHIP_F32) {
+            if (four) *reinterpret_cast<eh_f32x4u*>(p) = eh_f32x4u{v[0], v[1], v[2], v[3]};
+        } else {
+            if (four) *reinterpret_cast<eh_u32x2h*>(p) = eh_u32x2h{eh_pack2<DT>(v[0], v[1]), eh_pack2<DT>(v[2], v[3])};
+        }
+        const int at = n & 4, last = n & 6;
+        // (values read first, then chosen: a choice of places would keep v in memory)
+        const float v0 = v[0], v1 = v[1], v2 = v[2], v4 = v[4], v5 = v[5], v6 = v[6];
+        const float x0 = four ? v4 : v0, x1 = four ? v5 : v1;
+        float x = v0;
+        x = last == 2 ? v2 : x;
+        x = last == 4 ? v4 : x;
+        x = last == 6 ? v6 : x;
+        if (n & 2) {
+            p[at] = (T)x0;
+            p[at + 1] = (T)x1;
+        }
+        if (n & 1) p[last] = (T)x;
     }
 }
 
