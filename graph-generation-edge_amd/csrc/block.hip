@@ -275,7 +275,7 @@ template <int DH, int DZ> struct gn_grad {
 template <int DH, int DZ, bool LAYER, int TPR, bool TINY = false>
 __global__ __launch_bounds__(GN_THREADS(TPR), (TPR == GN_ROW ? 4 : GN_BWD_WAVES(DH))) void k_gn_bwd(gn_args A) {
     constexpr int RPB = TPR <= 64 ? 256 / TPR : 1;
-    constexpr bool AHEAD = DH != EDGEHIP_F32;                    // a row's requests a row ahead, where they fit the registers
+    constexpr bool AHEAD = DH != EDGEHIP_F32 && TPR > 64 && !LAYER;   // requests a row ahead, where they fit the registers
     extern __shared__ float par[];
     __shared__ float lds[64];
     __shared__ float fl[RPB > 1 ? 256 * 8 : 1];

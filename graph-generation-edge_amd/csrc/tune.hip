@@ -11,15 +11,18 @@
 // multiplied.
 //
 // Bound by HBM for many classes: 2 bytes a bf16 logit in, 2 out.  The one-pass form reads a row once, keeps it in
-// registers (64 values a thread) while its sum is taken, and writes its gradient; rows too long for that are read a
-// second time right after the first, from cache.  The log-probability and everything that follows from it is fp64, once
-// per row: its error would enter every value of the gradient, and gaps near 0 cancel in fp32; the exponentials are
-// fp32 (1e-7 relative each), their sum of many is better than each.  Sums over a sequence's rows are fp64, in a fixed order.
+// registers while its sum is taken, and writes its gradient; rows too long for that are read a second time right after
+// the first, from cache.  The log-probability and its differences (to old, to ref) are fp64, a few operations a row:
+// their error would enter every value of the gradient.  What follows from a difference is fp32 in forms that do not cancel,
+// the exponentials of a row are fp32 (1e-7 relative each), their sum is better than each.  Whether the clip binds is
+// decided on the logarithm in fp64.  Sums over a sequence's rows are fp64, in a fixed order.
 #include "common.h"
 #include "prof.h"
 #include "vec.h"
+#include <math.h>
 
-#define TN_KEEP 8                       // 8-value pieces of its row a thread keeps
+// 8-value pieces of its row a thread keeps (64 registers)
+#define TN_KEEP(DT) ((DT) == EDGEHIP_F32 ? 8 : 16)
 #define TN_LOG2E 1.44269504088896341f
 
 struct tn_rows {
@@ -30,15 +33,17 @@ struct tn_rows {
     // policy
     const float *old_logp, *adv, *ref;
     int adv_per_row;
-    float kl_coef; double lo, hi;       // 1 - lo, 1 + hi
+    float kl_coef, lo, hi;              // 1 - lo, 1 + hi
+    double ln_lo, ln_hi;                // their logarithms
     // per row
     float* logp;                        // log-probability (0 where the row does not count)
     double* logp64;                     // the same, for sums whose differences matter
     float* rowstat;                     // [R][2] max and 1 / sum
     float* term; float* kl; float* dterm; uint8_t* clipped;
     // per sequence
-    const double* scale;                // factor of dterm in the gradient
-    const float* coef;                  // per row instead: factor of (onehot - softmax)
+    const double* scale;                // factor of dterm in the gradient; NULL: weight[s], or each
+    const float* weight; double each;
+    double* part;                       // partial sums of the rows' terms (8 classes or less: made with the terms)
     void* dlogits;                      // dense [R][C]
 };
 
@@ -57,40 +62,71 @@ __device__ static inline int tn_seq(const int64_t* __restrict__ ptr, int S, int6
     return lo;
 }
 
-// exp(d) - 1 - d without cancellation near 0
-__device__ static inline double tn_kl(double d) {
-    if (fabs(d) < 0.125) {
-        double s = 1.0 / 39916800.0;                             // d^11 / 11!: next term 1e-19 of the first
-        s = s * d + 1.0 / 3628800.0;
-        s = s * d + 1.0 / 362880.0;
-        s = s * d + 1.0 / 40320.0;
-        s = s * d + 1.0 / 5040.0;
-        s = s * d + 1.0 / 720.0;
-        s = s * d + 1.0 / 120.0;
-        s = s * d + 1.0 / 24.0;
-        s = s * d + 1.0 / 6.0;
-        s = s * d + 0.5;
+__device__ static inline double tn_scale(const tn_rows& T, int seq) {
+    return T.scale ? T.scale[seq] : T.weight ? (double)T.weight[seq] : T.each;
+}
+
+// exp(d) - 1 - d, to a few ulp: its series (d^2 / 2 + ...; the term after the last is below 2^-25 of the first) near 0
+__device__ static inline float tn_kl(float d) {
+    if (fabsf(d) < 1.0f) {
+        float s = 1.0f / 479001600.0f;
+        s = s * d + 1.0f / 39916800.0f;
+        s = s * d + 1.0f / 3628800.0f;
+        s = s * d + 1.0f / 362880.0f;
+        s = s * d + 1.0f / 40320.0f;
+        s = s * d + 1.0f / 5040.0f;
+        s = s * d + 1.0f / 720.0f;
+        s = s * d + 1.0f / 120.0f;
+        s = s * d + 1.0f / 24.0f;
+        s = s * d + 1.0f / 6.0f;
+        s = s * d + 0.5f;
         return s * d * d;
     }
-    return d > 700.0 ? exp(d) : expm1(d) - d;                    // (an infinite gap is not NaN)
+    return d > 80.0f ? expf(d) : expf(d) - 1.0f - d;             // (an infinite gap is not NaN)
 }
 
 // the policy terms of one counted row; returns d term / d logp
-__device__ static inline double tn_policy(const tn_rows& T, int64_t r, int seq, double logp, double& term, double& kl, bool& cut) {
-    const double A = T.adv[T.adv_per_row ? r : seq];
-    const double rho = exp(logp - (double)T.old_logp[r]);
-    cut = A > 0.0 ? rho > T.hi : (A < 0.0 && rho < T.lo);
-    const double bound = A > 0.0 ? T.hi : T.lo;
+__device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, double logp, float& term, float& kl, bool& cut) {
+    const float A = T.adv[T.adv_per_row ? r : seq];
+    const double gain = logp - (double)T.old_logp[r];
+    const float rho = expf((float)gain);
+    cut = A > 0.0f ? gain > T.ln_hi : (A < 0.0f && gain < T.ln_lo);
+    const float bound = A > 0.0f ? T.hi : T.lo;
     term = -A * (cut ? bound : rho);
-    double d = cut ? 0.0 : -A * rho;
-    kl = 0.0;
+    float d = cut ? 0.0f : -A * rho;
+    kl = 0.0f;
     if (T.ref) {
-        const double gap = (double)T.ref[r] - logp;
+        const float gap = (float)((double)T.ref[r] - logp);
         kl = tn_kl(gap);
-        term += (double)T.kl_coef * kl;
-        d -= (double)T.kl_coef * (kl + gap);                     // exp(gap) - 1
+        term += T.kl_coef * kl;
+        d -= T.kl_coef * (kl + gap);                             // exp(gap) - 1
     }
     return d;
+}
+
+// Sums of v over the lanes of a wave that share a sequence (64 consecutive rows, a lane each; lanes that do not count have
+// v = 0, rows of no sequence g = -1): the last lane of a run writes them as partial (wave w, sequence g), at slot w + g.
+// Along the rows one of the two grows by one at each border, so the slots are distinct and waves + sequences of them are
+// enough.
+#define TN_WAVE 64
+__device__ static inline void tn_wave_part(double (&v)[4], int g, int64_t w, double* __restrict__ part) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int g2 = __shfl_up(g, o, 64);
+        const bool same = lane >= o && g2 == g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double u = __shfl_up(v[i], o, 64);
+            if (same) v[i] += u;
+        }
+    }
+    const int after = __shfl_down(g, 1, 64);
+    if (g >= 0 && (lane == 63 || after != g)) {
+        double* p = part + (w + g) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = v[i];
+    }
 }
 
 // max and sum over the TPR threads of a row: the running pair of a softmax, merged
@@ -141,26 +177,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     __shared__ float lds[2 * (TPR < 64 ? 1 : TPR / 64)];
     const int t = threadIdx.x % TPR;
     const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (TPR <= 64 && r >= T.R) return;                           // (TPR > 64: one row per block, none too many)
+    if (TPR > 1 && TPR <= 64 && r >= T.R) return;                // (TPR > 64: one row per block, none too many)
     const int C = T.C;
     const int64_t base = r * T.ld;
-    int64_t a;
-    const bool counts = tn_counts(T, r, a);
-    eh_raw8<DT> keep[TN_KEEP];
+    int64_t a = -1;
+    const bool counts = r < T.R && tn_counts(T, r, a);
+    constexpr int KEEP = TN_KEEP(DT);
+    eh_raw8<DT> keep[MODE == 2 && TPR > 1 ? KEEP : 1];
     float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
     float coef = 0.0f;
     const int full = C - 7;                                       // pieces starting below it are whole
-    const bool kept = MODE == 2 && C <= TPR * 8 * TN_KEEP;
+    const bool kept = MODE == 2 && TPR > 1 && C <= TPR * 8 * KEEP;
     if (MODE != 1) {
         if (counts) {
             if (kept) {
 #pragma unroll
-                for (int k = 0; k < TN_KEEP; ++k) {
+                for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
                     const int c = (k * TPR + t) * 8;
                     if (c < full) keep[k].load(reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits) + base + c);
                 }
 #pragma unroll
-                for (int k = 0; k < TN_KEEP; ++k) {
+                for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
                     const int c = (k * TPR + t) * 8;
                     float v[8];
                     if (c < full) { keep[k].get(v); tn_add8(m, s, v); }
@@ -175,40 +212,47 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
             }
             tn_row_merge<TPR>(m, s, lds);                         // (a row counts for all of its threads or none)
         }
-        double logp = 0.0, d = 0.0, term = 0.0, kl = 0.0;
+        double logp = 0.0;
+        float d = 0.0f, term = 0.0f, kl = 0.0f;
         bool cut = false;
-        int seq = 0;
+        int seq = -1;
         if (counts) {
             const float xa = (float)reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits)[base + a];
-            logp = (double)xa - (double)m - log((double)s);
+            logp = (double)xa - (double)m - (TPR > 1 || T.logp64 ? log((double)s) : (double)logf(s));
             inv = 1.0f / s;
             if (T.old_logp) {
                 seq = tn_seq(T.seq_ptr, T.S, r);
                 d = tn_policy(T, r, seq, logp, term, kl, cut);
-                if (MODE == 2) coef = (float)(d * T.scale[seq]);
+                if (MODE == 2) coef = (float)((double)d * tn_scale(T, seq));
             }
         }
-        if (t == 0) {
+        if (t == 0 && r < T.R) {
             if (T.logp) T.logp[r] = (float)logp;
             if (T.logp64) T.logp64[r] = logp;
             if (T.rowstat) { T.rowstat[2 * r] = m; T.rowstat[2 * r + 1] = inv; }
-            if (T.term) {
-                T.term[r] = (float)term;
-                T.kl[r] = (float)kl;
+            if (T.dterm) T.dterm[r] = d;
+            if (T.term && TPR > 1) {
+                T.term[r] = term;
+                T.kl[r] = kl;
                 T.clipped[r] = cut;
-                if (T.dterm) T.dterm[r] = (float)d;
             }
         }
+        if (TPR == 1 && T.old_logp) {
+            double v[4] = {(double)term, (double)kl, cut ? 1.0 : 0.0, counts ? 1.0 : 0.0};
+            if (!counts && r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S]) seq = tn_seq(T.seq_ptr, T.S, r);
+            tn_wave_part(v, seq, r / TN_WAVE, T.part);
+        }
+        if (TPR == 1 && r >= T.R) return;
     } else if (counts) {
         m = T.rowstat[2 * r];
         inv = T.rowstat[2 * r + 1];
         const int seq = tn_seq(T.seq_ptr, T.S, r);
-        coef = T.dterm ? (float)((double)T.dterm[r] * T.scale[seq]) : (float)T.scale[seq];
+        coef = (float)(T.dterm ? (double)T.dterm[r] * tn_scale(T, seq) : tn_scale(T, seq));
     }
-    if (MODE != 0) {
+    if (MODE != 0 && (TPR > 1 || r < T.R)) {
         const float f = -coef * inv;
 #pragma unroll
-        for (int k = 0; k < (MODE == 2 ? TN_KEEP : 1); ++k) {
+        for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
             for (int c = (k * TPR + t) * 8; c < C; c += TPR * 8) {
                 float v[8];
                 if (!counts) {
@@ -232,45 +276,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     }
 }
 
-// ---- sums over the rows of a sequence ----------------------------------------------------------------------------
-// A block owns TN_CHUNK consecutive rows and writes one partial per (block c, sequence g) it meets, at slot c + g: along
-// the rows one of the two grows by one at each border, so the slots are distinct and blocks + S of them are enough.
-// WHAT 0: counted rows; 1: policy (term, kl, clipped, count); 2: preference (logp - ref)
-#define TN_CHUNK 2048
+// ---- sums over the rows of a sequence (tn_wave_part), a lane a row ----------------------------------------------------
+// WHAT 0: counted rows; 1: policy (term, kl, clipped, count); 2: preference (logp - ref, count)
 template <int WHAT>
-__global__ __launch_bounds__(256) void k_tn_part(tn_rows T, double* __restrict__ part) {
-    __shared__ double red[4][4];
-    const int64_t r0 = (int64_t)blockIdx.x * TN_CHUNK;
-    int64_t r1 = r0 + TN_CHUNK < T.R ? r0 + TN_CHUNK : T.R;
-    if (r1 > T.seq_ptr[T.S]) r1 = T.seq_ptr[T.S];
-    if (r0 >= r1) return;
-    int g = tn_seq(T.seq_ptr, T.S, r0);
-    for (int64_t a = r0; a < r1;) {
-        while (g < T.S - 1 && T.seq_ptr[g + 1] <= a) ++g;
-        int64_t b = T.seq_ptr[g + 1];
-        if (b > r1 || g == T.S - 1) b = r1;
-        double v[4] = {0.0, 0.0, 0.0, 0.0};
-        for (int64_t r = a + threadIdx.x; r < b; r += 256) {
-            int64_t cls;
-            if (!tn_counts(T, r, cls)) continue;
-            v[3] += 1.0;
-            if (WHAT == 1) { v[0] += T.term[r]; v[1] += T.kl[r]; v[2] += T.clipped[r]; }
-            if (WHAT == 2) v[0] += T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
+__global__ __launch_bounds__(256) void k_tn_part(tn_rows T) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    int g = -1;
+    if (r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S]) {
+        g = tn_seq(T.seq_ptr, T.S, r);
+        int64_t cls;
+        if (tn_counts(T, r, cls)) {
+            v[3] = 1.0;
+            if (WHAT == 1) { v[0] = T.term[r]; v[1] = T.kl[r]; v[2] = T.clipped[r]; }
+            if (WHAT == 2) v[0] = T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], o, 64);
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) red[threadIdx.x >> 6][i] = v[i];
-        }
-        __syncthreads();
-        if (threadIdx.x < 4) part[((int64_t)blockIdx.x + g) * 4 + threadIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
-        a = b;
     }
+    tn_wave_part(v, g, r / TN_WAVE, T.part);
 }
 
 struct tn_final {
@@ -282,14 +304,15 @@ struct tn_final {
     // preference
     int kind; double beta, smooth; float* margin;
 };
-__device__ static inline void tn_total(const tn_final& F, int g, double (&v)[4]) {
+// totals of sequence g in every thread of the block (256)
+__device__ static inline void tn_total(const tn_final& F, int g, double (&v)[4], double (&red)[4][4]) {
     int64_t a = F.seq_ptr[g], b = F.seq_ptr[g + 1];
     if (a < 0) a = 0;
     if (b > F.R) b = F.R;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = 0.0;
     if (a < b) {
-        for (int64_t c = a / TN_CHUNK + (threadIdx.x & 63); c <= (b - 1) / TN_CHUNK; c += 64) {
+        for (int64_t c = a / TN_WAVE + threadIdx.x; c <= (b - 1) / TN_WAVE; c += 256) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += F.part[(c + g) * 4 + i];
         }
@@ -299,13 +322,22 @@ __device__ static inline void tn_total(const tn_final& F, int g, double (&v)[4])
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], o, 64);
     }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[threadIdx.x >> 6][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
 }
-// one wave per sequence.  PASS 0: the gradient's scale from the counted rows; 1: the losses
+// a block a sequence.  PASS 0: the gradient's scale from the counted rows; 1: the losses
 template <int PASS>
-__global__ __launch_bounds__(64) void k_tn_policy_final(tn_final F) {
+__global__ __launch_bounds__(256) void k_tn_policy_final(tn_final F) {
+    __shared__ double red[4][4];
     const int g = blockIdx.x;
     double v[4];
-    tn_total(F, g, v);
+    tn_total(F, g, v, red);
     if (threadIdx.x) return;
     const double inv = F.mean ? 1.0 / (v[3] > 0.0 ? v[3] : 1.0) : 1.0;
     if (F.scale) F.scale[g] = (F.weight ? (double)F.weight[g] : F.each) * inv;
@@ -315,12 +347,13 @@ __global__ __launch_bounds__(64) void k_tn_policy_final(tn_final F) {
         F.clipped[g] = (int32_t)v[2];
     }
 }
-// one wave per pair: chosen sequence g, rejected sequence g + pairs
-__global__ __launch_bounds__(64) void k_tn_pref_final(tn_final F) {
+// a block a pair: chosen sequence g, rejected sequence g + pairs
+__global__ __launch_bounds__(256) void k_tn_pref_final(tn_final F) {
+    __shared__ double red[4][4];
     const int g = blockIdx.x, P = F.S / 2;
     double c[4], r[4];
-    tn_total(F, g, c);
-    tn_total(F, g + P, r);
+    tn_total(F, g, c, red);
+    tn_total(F, g + P, r, red);
     if (threadIdx.x) return;
     const double ic = F.mean ? 1.0 / (c[3] > 0.0 ? c[3] : 1.0) : 1.0, ir = F.mean ? 1.0 / (r[3] > 0.0 ? r[3] : 1.0) : 1.0;
     const double margin = c[0] * ic - r[0] * ir;
@@ -347,12 +380,10 @@ __global__ __launch_bounds__(64) void k_tn_pref_final(tn_final F) {
 template <int MODE>
 static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
     if (T.R == 0) return EDGEHIP_OK;
-    // threads of a row: eight values each at least, 64 at most while the row can be kept
-    int tpr = 1;
-    if (T.C > 8) tpr = 8;
-    if (T.C > 512) tpr = 64;
-    if (T.C > 4096) tpr = 256;
-    if (T.C > 16384) tpr = 1024;
+    // threads of a row: as few as can keep it whole, so that a CU has several rows in different phases (8192 x 32003 bf16,
+    // one pass: 1024 threads a row 382 us, 256 BENCH)
+    const int per = 8 * (dtype == EDGEHIP_F32 ? TN_KEEP(EDGEHIP_F32) : TN_KEEP(EDGEHIP_BF16));
+    const int tpr = T.C <= 8 ? 1 : T.C <= 512 ? 8 : T.C <= 4096 ? 64 : T.C <= 256 * per ? 256 : 1024;
     const int rpb = (tpr < 256 ? 256 : tpr) / tpr;
     const dim3 grid((unsigned)((T.R + rpb - 1) / rpb)), block(tpr < 256 ? 256 : tpr);
 #define TN_TPR(DT, N) case N: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, N, MODE>), grid, block, 0, s, T)); break;
@@ -383,7 +414,7 @@ static tn_rows tn_fill(const edgehip_logit_rows* Q) {
 struct tn_ws { double *scale, *part, *logp; float *term, *kl, *dterm, *stat; uint8_t* clipped; size_t bytes; };
 static tn_ws tn_layout(const edgehip_logit_rows* Q, void* ws) {
     tn_ws W;
-    const size_t R = (size_t)Q->rows, S = (size_t)Q->num_seqs, chunks = (R + TN_CHUNK - 1) / TN_CHUNK;
+    const size_t R = (size_t)Q->rows, S = (size_t)Q->num_seqs, chunks = (R + TN_WAVE - 1) / TN_WAVE;
     char* p = reinterpret_cast<char*>(ws);
     size_t o = 0;
     auto take = [&](size_t n) { char* q = p + o; o += (n + 15) & ~(size_t)15; return q; };
@@ -403,9 +434,9 @@ extern "C" size_t edgehip_tune_workspace_bytes(const edgehip_logit_rows* Q) {
 }
 
 template <int WHAT>
-static int tn_sum(const tn_rows& T, double* part, hipStream_t s) {
+static int tn_sum(const tn_rows& T, hipStream_t s) {
     if (T.R == 0) return EDGEHIP_OK;
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_part<WHAT>), dim3((unsigned)((T.R + TN_CHUNK - 1) / TN_CHUNK)), dim3(256), 0, s, T, part));
+    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_part<WHAT>), dim3((unsigned)((T.R + 255) / 256)), dim3(256), 0, s, T));
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -429,8 +460,10 @@ static int tn_policy_args(const edgehip_logit_rows* Q, const edgehip_policy* O, 
     W = tn_layout(Q, ws);
     T = tn_fill(Q);
     T.old_logp = O->old_logp; T.adv = O->advantage; T.ref = O->ref_logp; T.adv_per_row = O->advantage_per_row;
-    T.kl_coef = (float)O->kl_coef; T.lo = 1.0 - O->clip_lo; T.hi = 1.0 + O->clip_hi;
-    T.term = W.term; T.kl = W.kl; T.clipped = W.clipped;
+    T.kl_coef = (float)O->kl_coef; T.lo = (float)(1.0 - O->clip_lo); T.hi = (float)(1.0 + O->clip_hi);
+    T.ln_lo = O->clip_lo < 1.0 ? log1p(-O->clip_lo) : -HUGE_VAL; T.ln_hi = log1p(O->clip_hi);
+    T.term = W.term; T.kl = W.kl; T.clipped = W.clipped; T.part = W.part;
+    T.weight = O->weight; T.each = 1.0 / (double)Q->num_seqs;
     F = tn_final{};
     F.seq_ptr = Q->seq_ptr; F.R = Q->rows; F.S = Q->num_seqs; F.part = W.part;
     F.mean = O->mean; F.weight = O->weight; F.each = 1.0 / (double)Q->num_seqs;
@@ -445,9 +478,9 @@ extern "C" int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehi
     hipStream_t s = eh_stream(stream);
     T.logp = logp; T.rowstat = W.stat; T.dterm = W.dterm;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
-    TN_TRY(tn_sum<1>(T, W.part, s));
+    if (T.C > 8) TN_TRY(tn_sum<1>(T, s));                     // (narrower rows: the row kernel makes the partials)
     F.loss = loss; F.kl = kl; F.clipped = clipped;
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(64), 0, s, F));
+    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -457,10 +490,13 @@ extern "C" int edgehip_policy_loss_bwd(const edgehip_logit_rows* Q, const edgehi
     TN_TRY(tn_policy_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(Q->rows == 0 || dlogits);
     hipStream_t s = eh_stream(stream);
-    F.scale = W.scale;                          // the partial sums of the forward are still in the workspace
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<0>), dim3(F.S), dim3(64), 0, s, F));
-    EH_LAUNCH_CHECK();
-    T.rowstat = W.stat; T.dterm = W.dterm; T.scale = W.scale; T.dlogits = dlogits;
+    if (F.mean) {                               // the partial sums of the forward are still in the workspace
+        F.scale = W.scale;
+        T.scale = W.scale;
+        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<0>), dim3(F.S), dim3(256), 0, s, F));
+        EH_LAUNCH_CHECK();
+    }
+    T.rowstat = W.stat; T.dterm = W.dterm; T.dlogits = dlogits;
     return tn_launch<1>(Q->dtype, T, s);
 }
 extern "C" int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgehip_policy* O, float* loss, float* kl, int32_t* clipped,
@@ -469,15 +505,18 @@ extern "C" int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgeh
     TN_TRY(tn_policy_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(loss && kl && clipped && (Q->rows == 0 || dlogits));
     hipStream_t s = eh_stream(stream);
-    F.scale = W.scale;
-    TN_TRY(tn_sum<0>(T, W.part, s));
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<0>), dim3(F.S), dim3(64), 0, s, F));
-    EH_LAUNCH_CHECK();
-    T.logp = logp; T.scale = W.scale; T.dlogits = dlogits;
+    if (F.mean) {                               // a mean needs the number of counted rows before the gradient
+        TN_TRY(tn_sum<0>(T, s));
+        F.scale = W.scale;
+        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<0>), dim3(F.S), dim3(256), 0, s, F));
+        EH_LAUNCH_CHECK();
+        T.scale = W.scale;
+    }
+    T.logp = logp; T.dlogits = dlogits;
     TN_TRY(tn_launch<2>(Q->dtype, T, s));
-    TN_TRY(tn_sum<1>(T, W.part, s));
+    if (T.C > 8) TN_TRY(tn_sum<1>(T, s));
     F.scale = nullptr; F.loss = loss; F.kl = kl; F.clipped = clipped;
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(64), 0, s, F));
+    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -490,7 +529,7 @@ static int tn_pref_args(const edgehip_logit_rows* Q, const edgehip_preference* O
     EH_CHECK_ARG(ws && ((uintptr_t)ws & 15) == 0);
     W = tn_layout(Q, ws);
     T = tn_fill(Q);
-    T.ref = O->ref_logp;
+    T.ref = O->ref_logp; T.part = W.part;
     F = tn_final{};
     F.seq_ptr = Q->seq_ptr; F.R = Q->rows; F.S = Q->num_seqs; F.part = W.part;
     F.mean = O->mean; F.weight = O->weight; F.each = 2.0 / (double)Q->num_seqs;
@@ -505,9 +544,9 @@ extern "C" int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const ed
     hipStream_t s = eh_stream(stream);
     T.logp64 = W.logp; T.rowstat = W.stat;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
-    TN_TRY(tn_sum<2>(T, W.part, s));
+    TN_TRY(tn_sum<2>(T, s));
     F.loss = loss; F.margin = margin;
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_tn_pref_final, dim3(F.S / 2), dim3(64), 0, s, F));
+    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_tn_pref_final, dim3(F.S / 2), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -518,7 +557,7 @@ extern "C" int edgehip_preference_loss_bwd(const edgehip_logit_rows* Q, const ed
     EH_CHECK_ARG(Q->rows == 0 || dlogits);
     hipStream_t s = eh_stream(stream);
     F.scale = W.scale;
-    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_tn_pref_final, dim3(F.S / 2), dim3(64), 0, s, F));
+    EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_tn_pref_final, dim3(F.S / 2), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
     T.rowstat = W.stat; T.scale = W.scale; T.dlogits = dlogits;
     return tn_launch<1>(Q->dtype, T, s);
