@@ -104,28 +104,53 @@ __device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, d
     return d;
 }
 
-// Sums of v over the lanes of a wave that share a sequence (64 consecutive rows, a lane each; lanes that do not count have
-// v = 0, rows of no sequence g = -1): the last lane of a run writes them as partial (wave w, sequence g), at slot w + g.
-// Along the rows one of the two grows by one at each border, so the slots are distinct and waves + sequences of them are
-// enough.
+// The sequence of this lane's row r (64 consecutive rows a wave), -1 where it lies in none.  Where the wave's first and last
+// row lie in one sequence - most waves - the search is done once, by the scalar unit.
+__device__ static inline int tn_lane_seq(const tn_rows& T, int64_t r) {
+    const int64_t first = ((int64_t)__builtin_amdgcn_readfirstlane((int)(r >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)r);
+    if (first >= T.seq_ptr[0] && first < T.seq_ptr[T.S]) {
+        const int g = tn_seq(T.seq_ptr, T.S, first);
+        if (first + 63 < T.seq_ptr[g + 1] && first + 63 < T.R) return g;
+    }
+    return r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S] ? tn_seq(T.seq_ptr, T.S, r) : -1;
+}
+
+// Sums over the lanes of a wave that share a sequence (g from tn_lane_seq; lanes that do not count have zeros): NV values,
+// and how many lanes have `cut` and `counts`.  The last lane of a run writes them as partial (wave w, sequence g), at slot
+// w + g: along the rows one of the two grows by one at each border, so the slots are distinct and waves + sequences of
+// them are enough.
 #define TN_WAVE 64
-__device__ static inline void tn_wave_part(double (&v)[4], int g, int64_t w, double* __restrict__ part) {
+template <int NV>
+__device__ static inline void tn_wave_part(double (&v)[NV], bool cut, bool counts, int g, int64_t w, double* __restrict__ part) {
     const int lane = threadIdx.x & 63;
+    const int before = __shfl_up(g, 1, 64), after = __shfl_down(g, 1, 64);
+    const uint64_t starts = __ballot(lane == 0 || before != g);
+    // lanes of this lane's run up to itself
+    const uint64_t upto = ~0ull >> (63 - lane), run = upto & ~((1ull << (63 - __builtin_clzll(starts & upto))) - 1);
+    const uint64_t cuts = __ballot(cut), all = __ballot(counts);
+    if (starts == 1) {                                           // one run: any order of pairs
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int g2 = __shfl_up(g, o, 64);
-        const bool same = lane >= o && g2 == g;
+        for (int o = 1; o < 64; o <<= 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double u = __shfl_up(v[i], o, 64);
-            if (same) v[i] += u;
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o, 64);
+        }
+    } else {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const bool same = lane >= o && (run >> (lane >= o ? lane - o : 0) & 1);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const double u = __shfl_up(v[i], o, 64);
+                if (same) v[i] += u;
+            }
         }
     }
-    const int after = __shfl_down(g, 1, 64);
     if (g >= 0 && (lane == 63 || after != g)) {
         double* p = part + (w + g) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = v[i];
+        p[0] = NV > 0 ? v[0] : 0.0;
+        p[1] = NV > 1 ? v[NV - 1] : 0.0;
+        p[2] = (double)__popcll(cuts & run);
+        p[3] = (double)__popcll(all & run);
     }
 }
 
@@ -216,12 +241,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         float d = 0.0f, term = 0.0f, kl = 0.0f;
         bool cut = false;
         int seq = -1;
+        if (TPR == 1 && T.old_logp) seq = tn_lane_seq(T, r);
         if (counts) {
             const float xa = (float)reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits)[base + a];
             logp = (double)xa - (double)m - (TPR > 1 || T.logp64 ? log((double)s) : (double)logf(s));
             inv = 1.0f / s;
             if (T.old_logp) {
-                seq = tn_seq(T.seq_ptr, T.S, r);
+                if (TPR > 1) seq = tn_seq(T.seq_ptr, T.S, r);
                 d = tn_policy(T, r, seq, logp, term, kl, cut);
                 if (MODE == 2) coef = (float)((double)d * tn_scale(T, seq));
             }
@@ -238,9 +264,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
             }
         }
         if (TPR == 1 && T.old_logp) {
-            double v[4] = {(double)term, (double)kl, cut ? 1.0 : 0.0, counts ? 1.0 : 0.0};
-            if (!counts && r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S]) seq = tn_seq(T.seq_ptr, T.S, r);
-            tn_wave_part(v, seq, r / TN_WAVE, T.part);
+            double v[2] = {(double)term, (double)kl};
+            tn_wave_part<2>(v, cut, counts, seq, r / TN_WAVE, T.part);
         }
         if (TPR == 1 && r >= T.R) return;
     } else if (counts) {
@@ -281,18 +306,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
 template <int WHAT>
 __global__ __launch_bounds__(256) void k_tn_part(tn_rows T) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    double v[4] = {0.0, 0.0, 0.0, 0.0};
-    int g = -1;
-    if (r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S]) {
-        g = tn_seq(T.seq_ptr, T.S, r);
-        int64_t cls;
-        if (tn_counts(T, r, cls)) {
-            v[3] = 1.0;
-            if (WHAT == 1) { v[0] = T.term[r]; v[1] = T.kl[r]; v[2] = T.clipped[r]; }
-            if (WHAT == 2) v[0] = T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
-        }
+    const int g = tn_lane_seq(T, r);
+    int64_t cls;
+    const bool counts = g >= 0 && tn_counts(T, r, cls);
+    double v[WHAT == 1 ? 2 : 1] = {0.0};
+    bool cut = false;
+    if (counts) {
+        if (WHAT == 1) { v[0] = T.term[r]; v[WHAT == 1] = T.kl[r]; cut = T.clipped[r]; }
+        if (WHAT == 2) v[0] = T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
     }
-    tn_wave_part(v, g, r / TN_WAVE, T.part);
+    tn_wave_part(v, cut, counts, g, r / TN_WAVE, T.part);
 }
 
 struct tn_final {
