@@ -154,11 +154,25 @@ __device__ static inline void tn_wave_part(double (&v)[NV], bool cut, bool count
     }
 }
 
+// exp(x), x <= 0 or NaN.  The fp32 constant log2(e) alone is 1.3e-8 off: every term of a row would be off to the same side by
+// that times |x|, and a preference's margin is the difference of hundreds of such rows.  With the constant's second part the
+// error of a term is that of rounding x log2(e), to either side; many terms average it.  FEW: rows of few classes have no
+// many, there the whole part is split off first and a term is right to 2 ulp (twice the work).
+template <bool FEW>
+__device__ static inline float tn_exp(float x) {
+    constexpr float HI = 1.44269502162933349609f, LO = 1.92596298909109e-8f;
+    if (!FEW) return __builtin_amdgcn_exp2f(__builtin_fmaf(x, HI, x * LO));
+    x = x < -150.0f ? -150.0f : x;
+    const float n = rintf(x * HI);
+    const float f = __builtin_fmaf(x, LO, __builtin_fmaf(x, HI, -n));
+    return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
+
 // max and sum over the TPR threads of a row: the running pair of a softmax, merged
 __device__ static inline void tn_merge(float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2);
     // equal (also both -inf): no exponent of a difference of infinities
-    s = (m == top ? s : s * __builtin_amdgcn_exp2f((m - top) * TN_LOG2E)) + (m2 == top ? s2 : s2 * __builtin_amdgcn_exp2f((m2 - top) * TN_LOG2E));
+    s = (m == top ? s : s * tn_exp<true>(m - top)) + (m2 == top ? s2 : s2 * tn_exp<true>(m2 - top));
     m = top;
 }
 template <int TPR>
@@ -180,16 +194,17 @@ __device__ static inline void tn_row_merge(float& m, float& s, float* lds) {
 }
 
 // eight more values into the running pair.  NaN: the sum becomes NaN and stays it.
+template <bool FEW>
 __device__ static inline void tn_add8(float& m, float& s, const float (&v)[8]) {
     float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
     top = fmaxf(top, m);
-    if (top > m) { s *= __builtin_amdgcn_exp2f((m - top) * TN_LOG2E); m = top; }     // m = -inf: s is 0 (or NaN) before
+    if (top > m) { s *= tn_exp<FEW>(m - top); m = top; }     // m = -inf: s is 0 (or NaN) before
     const float base = m == -__builtin_inff() ? 0.0f : m;                            // all -inf so far: exp(-inf) = 0
     float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        a += __builtin_amdgcn_exp2f((v[i] - base) * TN_LOG2E);
-        b += __builtin_amdgcn_exp2f((v[i + 1] - base) * TN_LOG2E);
+        a += tn_exp<FEW>(v[i] - base);
+        b += tn_exp<FEW>(v[i + 1] - base);
     }
     s += a + b;
 }
@@ -225,14 +240,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
                 for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
                     const int c = (k * TPR + t) * 8;
                     float v[8];
-                    if (c < full) { keep[k].get(v); tn_add8(m, s, v); }
-                    else if (c < C) { eh_load8<DT>(T.logits, base + c, C - c, v, -__builtin_inff()); tn_add8(m, s, v); }
+                    if (c < full) { keep[k].get(v); tn_add8<(TPR <= 64)>(m, s, v); }
+                    else if (c < C) { eh_load8<DT>(T.logits, base + c, C - c, v, -__builtin_inff()); tn_add8<(TPR <= 64)>(m, s, v); }
                 }
             } else {
                 for (int c = t * 8; c < C; c += TPR * 8) {
                     float v[8];
                     eh_load8<DT>(T.logits, base + c, C - c, v, -__builtin_inff());
-                    tn_add8(m, s, v);
+                    tn_add8<(TPR <= 64)>(m, s, v);
                 }
             }
             tn_row_merge<TPR>(m, s, lds);                         // (a row counts for all of its threads or none)
