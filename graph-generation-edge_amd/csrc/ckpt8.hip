@@ -567,7 +567,7 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
         p.nt = eh_cdiv((int64_t)N * K, 256);
         p.kt = 1;
     }
-    const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 255) / 256;
+    const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 63) / 64;
     const int64_t room = p.tile == 256 ? 256 : 512;      // blocks the chip holds at once
     int64_t s = tiles >= room ? 1 : room / tiles;
     if (s > most) s = most;

@@ -574,12 +574,8 @@ static int tn_pref_args(const edgehip_logit_rows* Q, const edgehip_preference* O
     F.kind = O->kind; F.beta = O->beta; F.smooth = O->label_smoothing;
     return EDGEHIP_OK;
 }
-extern "C" int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const edgehip_preference* O, float* loss, float* margin,
-                                           void* ws, size_t ws_bytes, void* stream) {
-    tn_rows T; tn_final F; tn_ws W;
-    TN_TRY(tn_pref_args(Q, O, T, F, W, ws, ws_bytes));
+static int tn_pref_fwd(const edgehip_logit_rows* Q, tn_rows& T, tn_final& F, tn_ws& W, float* loss, float* margin, hipStream_t s) {
     EH_CHECK_ARG(loss && margin);
-    hipStream_t s = eh_stream(stream);
     T.logp64 = W.logp; T.rowstat = W.stat;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
     TN_TRY(tn_sum<2>(T, s));
@@ -587,6 +583,22 @@ extern "C" int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const ed
     EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_tn_pref_final, dim3(F.S / 2), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
+}
+extern "C" int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const edgehip_preference* O, float* loss, float* margin,
+                                           void* ws, size_t ws_bytes, void* stream) {
+    tn_rows T; tn_final F; tn_ws W;
+    TN_TRY(tn_pref_args(Q, O, T, F, W, ws, ws_bytes));
+    return tn_pref_fwd(Q, T, F, W, loss, margin, eh_stream(stream));
+}
+extern "C" int edgehip_preference_loss_grad(const edgehip_logit_rows* Q, const edgehip_preference* O, float* loss, float* margin,
+                                            void* dlogits, void* ws, size_t ws_bytes, void* stream) {
+    tn_rows T; tn_final F; tn_ws W;
+    TN_TRY(tn_pref_args(Q, O, T, F, W, ws, ws_bytes));
+    EH_CHECK_ARG(Q->rows == 0 || dlogits);
+    F.scale = W.scale;
+    TN_TRY(tn_pref_fwd(Q, T, F, W, loss, margin, eh_stream(stream)));
+    T.logp64 = nullptr; T.scale = W.scale; T.dlogits = dlogits;
+    return tn_launch<1>(Q->dtype, T, eh_stream(stream));
 }
 extern "C" int edgehip_preference_loss_bwd(const edgehip_logit_rows* Q, const edgehip_preference* O, void* dlogits, void* ws,
                                            size_t ws_bytes, void* stream) {

@@ -93,9 +93,9 @@ def _fwd(G, h, z, want_stats):
     h_out = torch.empty_like(h)
     y = torch.empty_like(z) if G.pre else None
     stats = torch.empty((G.rows, 4), dtype=torch.float32, device=h.device) if want_stats else None
-    with capi.device_of(h):
+    with capi.on_device_of(h) as stream:
         capi.check(lib.edgehip_gate_norm_fwd(byref(G), h.data_ptr(), z.data_ptr(), h_out.data_ptr(), capi.ptr(y),
-                                             capi.ptr(stats), capi.stream_ptr()), 'gate_norm_fwd')
+                                             capi.ptr(stats), stream), 'gate_norm_fwd')
     return h_out, y, stats
 
 
@@ -123,11 +123,11 @@ def _bwd(G, dh_out, dy, h, z, stats, gate, like, want):
     nbytes = lib.edgehip_gate_norm_workspace_bytes(byref(G))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     p = {k: v.data_ptr() for k, v in out.items()}
-    with capi.device_of(h):
+    with capi.on_device_of(h) as stream:
         capi.check(lib.edgehip_gate_norm_bwd(byref(G), capi.ptr(dh_out), capi.ptr(dy), h.data_ptr(), z.data_ptr(),
                                              stats.data_ptr(), p['dh'], p['dz'], p.get('dgate'), p.get('dw_pre'),
                                              p.get('db_pre'), p.get('dw_post'), p.get('db_post'), ws.data_ptr(), nbytes,
-                                             capi.stream_ptr()), 'gate_norm_bwd')
+                                             stream), 'gate_norm_bwd')
     return out
 
 

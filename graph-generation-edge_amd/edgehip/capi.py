@@ -160,6 +160,7 @@ EXPORTS = {
     'edgehip_policy_loss_grad': [C.POINTER(LogitRows), C.POINTER(Policy), vp, vp, vp, vp, vp, vp, C.c_size_t, vp],
     'edgehip_preference_loss_fwd': [C.POINTER(LogitRows), C.POINTER(Preference), vp, vp, vp, C.c_size_t, vp],
     'edgehip_preference_loss_bwd': [C.POINTER(LogitRows), C.POINTER(Preference), vp, vp, C.c_size_t, vp],
+    'edgehip_preference_loss_grad': [C.POINTER(LogitRows), C.POINTER(Preference), vp, vp, vp, vp, C.c_size_t, vp],
 }
 SIZE_EXPORTS = {
     'edgehip_gate_norm_workspace_bytes': [C.POINTER(GateNorm)],
@@ -251,12 +252,17 @@ def stream_ptr():
 
 
 # ---- argument checks shared by the operators over several types (block, ckpt8, tune) ----------------------
+# (plain attribute tests and no context manager where the device is current already: for a single token these cost as much
+# as the kernel)
 F32, BF16, F16 = 0, 1, 2
+_CODES = {}
 
 
 def dtype_code(what, name, t):
-    import torch
-    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(t.dtype)
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    code = _CODES.get(t.dtype)
     if code is None:
         raise ValueError(f'{what}: {name} must be fp32, bf16 or fp16, got {t.dtype}')
     return code
@@ -272,10 +278,24 @@ def on_gpu(what, t):
         raise ValueError(f'{what}: the tensors must be on a GPU (there is no CPU path), got {t.device}')
 
 
-def device_of(t):
-    """with device_of(t): the tensor's GPU is current, so that `stream_ptr` names a stream of it."""
-    import torch
-    return torch.cuda.device(t.device)
+class on_device_of:
+    """with on_device_of(t) as s: t's GPU is current and s is its current stream."""
+    __slots__ = ('index', 'before')
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        import torch
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch.cuda.set_device(self.before)
 
 
 # One pool of side streams per device for everything in this package (the sampler's sub-batch streams, the training

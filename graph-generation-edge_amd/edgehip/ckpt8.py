@@ -39,9 +39,9 @@ class Packed8:
         capi.on_gpu('unpack8', x)
         if x.numel():
             rows, k = _rows(x)
-            with capi.device_of(x):
+            with capi.on_device_of(x) as stream:
                 capi.check(lib.edgehip_unpack8(code, self.codes.data_ptr(), self.exps.data_ptr(), rows, k, x.data_ptr(),
-                                               capi.stream_ptr()), 'unpack8')
+                                               stream), 'unpack8')
         return x
 
 
@@ -75,9 +75,9 @@ def pack8(x):
     kept = _new(x)
     if x.numel():
         rows, k = _rows(x)
-        with capi.device_of(x):
+        with capi.on_device_of(x) as stream:
             capi.check(lib.edgehip_pack8(code, x.data_ptr(), rows, k, kept.codes.data_ptr(), kept.exps.data_ptr(),
-                                         capi.stream_ptr()), 'pack8')
+                                         stream), 'pack8')
     return kept
 
 
@@ -89,9 +89,9 @@ def act8_fwd(x, kind='silu'):
     y, kept = torch.empty_like(x), _new(x)
     if x.numel():
         rows, k = _rows(x)
-        with capi.device_of(x):
+        with capi.on_device_of(x) as stream:
             capi.check(lib.edgehip_act8_fwd(code, kc, x.data_ptr(), rows, k, y.data_ptr(), kept.codes.data_ptr(),
-                                            kept.exps.data_ptr(), capi.stream_ptr()), what)
+                                            kept.exps.data_ptr(), stream), what)
     return y, kept
 
 
@@ -115,9 +115,9 @@ def act8_bwd(dy, kept, kind='silu'):
     dx = torch.empty_like(dy)
     if dy.numel():
         rows, k = _rows(dy)
-        with capi.device_of(dy):
+        with capi.on_device_of(dy) as stream:
             capi.check(lib.edgehip_act8_bwd(code, kc, dy.data_ptr(), kept.codes.data_ptr(), kept.exps.data_ptr(), rows, k,
-                                            dx.data_ptr(), capi.stream_ptr()), what)
+                                            dx.data_ptr(), stream), what)
     return dx
 
 
@@ -138,9 +138,9 @@ def linear8_bwd_weight(dy, kept, bias=True):
     if nbytes == 0:
         raise ValueError(f'{what}: layers of up to {1 << 22} inputs and outputs')
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
-    with capi.device_of(dy):
+    with capi.on_device_of(dy) as stream:
         capi.check(lib.edgehip_linear8_bwd_weight(code, dy.data_ptr(), kept.codes.data_ptr(), kept.exps.data_ptr(), m, n, k,
-                                                  dw.data_ptr(), capi.ptr(db), ws.data_ptr(), nbytes, capi.stream_ptr()), what)
+                                                  dw.data_ptr(), capi.ptr(db), ws.data_ptr(), nbytes, stream), what)
     return dw, db
 
 
@@ -180,10 +180,10 @@ class _Linear8(Function):
             y = torch.empty((x.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
             if x.shape[0]:
                 wc = w.contiguous()
-                with capi.device_of(x):
+                with capi.on_device_of(x) as stream:
                     capi.check(lib.edgehip_linear_fwd(x.data_ptr(), x.shape[0], w.shape[1], wc.data_ptr(),
                                                       capi.ptr(b.contiguous() if b is not None else None), w.shape[0], 0,
-                                                      y.data_ptr(), capi.stream_ptr()), 'linear_fwd')
+                                                      y.data_ptr(), stream), 'linear_fwd')
         else:
             y = torch.nn.functional.linear(x, w, b)
         ctx.save_for_backward(w, kept and kept.codes, kept and kept.exps)
@@ -202,9 +202,9 @@ class _Linear8(Function):
                 if dy.shape[0]:
                     wt = torch.empty(k * n, dtype=torch.float32, device=dy.device)
                     wc = w.contiguous()
-                    with capi.device_of(dy):
+                    with capi.on_device_of(dy) as stream:
                         capi.check(lib.edgehip_linear_bwd_input(dy.data_ptr(), dy.shape[0], n, wc.data_ptr(), k, wt.data_ptr(),
-                                                                dx.data_ptr(), capi.stream_ptr()), 'linear_bwd_input')
+                                                                dx.data_ptr(), stream), 'linear_bwd_input')
             else:
                 dx = torch.matmul(dy, w)
         want_db = ctx.has_bias and ctx.needs_input_grad[2]

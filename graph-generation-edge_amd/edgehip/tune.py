@@ -77,8 +77,8 @@ def row_logp(logits, taken, mask=None):
     Q, keep = _describe('row_logp', logits, taken, None, mask)
     capi.on_gpu('row_logp', logits)
     out = torch.empty(Q.rows, dtype=torch.float32, device=logits.device)
-    with capi.device_of(logits):
-        capi.check(lib.edgehip_row_logp(byref(Q), out.data_ptr(), capi.stream_ptr()), 'row_logp')
+    with capi.on_device_of(logits) as stream:
+        capi.check(lib.edgehip_row_logp(byref(Q), out.data_ptr(), stream), 'row_logp')
     return out
 
 
@@ -129,10 +129,10 @@ def policy_loss_grad(logits, taken, old_logp, advantage, seq_ptr, *, ref_logp=No
     loss, kl, clipped, logp = _policy_out(Q, dev)
     dlogits = torch.empty((Q.rows, Q.classes), dtype=logits.dtype, device=dev)
     ws = _workspace(Q, dev)
-    with capi.device_of(logits):
+    with capi.on_device_of(logits) as stream:
         capi.check(lib.edgehip_policy_loss_grad(byref(Q), byref(O), loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(),
                                                 logp.data_ptr(), dlogits.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                capi.stream_ptr()), 'policy_loss_grad')
+                                                stream), 'policy_loss_grad')
     return PolicyGrad(loss, kl, clipped, logp, dlogits)
 
 
@@ -142,9 +142,9 @@ class _PolicyLoss(Function):
         Q, O, keep = _policy_args('policy_loss', logits, taken, old_logp, advantage, seq_ptr, ref_logp, mask, None, **opts)
         loss, kl, clipped, logp = _policy_out(Q, logits.device)
         ws = _workspace(Q, logits.device)
-        with capi.device_of(logits):
+        with capi.on_device_of(logits) as stream:
             capi.check(lib.edgehip_policy_loss_fwd(byref(Q), byref(O), loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(),
-                                                   logp.data_ptr(), ws.data_ptr(), ws.numel(), capi.stream_ptr()),
+                                                   logp.data_ptr(), ws.data_ptr(), ws.numel(), stream),
                        'policy_loss_fwd')
         ctx.save_for_backward(logits, taken, old_logp, advantage, seq_ptr, ref_logp, mask, ws)
         ctx.opts = opts
@@ -157,9 +157,9 @@ class _PolicyLoss(Function):
         Q, O, keep = _policy_args('policy_loss', logits, taken, old_logp, advantage, seq_ptr, ref_logp, mask,
                                   dloss.float().contiguous(), **ctx.opts)
         dlogits = torch.empty((Q.rows, Q.classes), dtype=logits.dtype, device=logits.device)
-        with capi.device_of(logits):
+        with capi.on_device_of(logits) as stream:
             capi.check(lib.edgehip_policy_loss_bwd(byref(Q), byref(O), dlogits.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                   capi.stream_ptr()), 'policy_loss_bwd')
+                                                   stream), 'policy_loss_bwd')
         return (dlogits,) + (None,) * 7
 
 
@@ -187,19 +187,19 @@ def _preference_args(what, logits, taken, seq_ptr, ref_logp, mask, weight, beta,
     return Q, O, keep + (ref_logp, weight)
 
 
-def _preference_fwd(Q, O, dev):
+def _preference_fwd(Q, O, dev, stream):
     loss = torch.empty(Q.num_seqs // 2, dtype=torch.float32, device=dev)
     margin = torch.empty_like(loss)
     ws = _workspace(Q, dev)
     capi.check(lib.edgehip_preference_loss_fwd(byref(Q), byref(O), loss.data_ptr(), margin.data_ptr(), ws.data_ptr(), ws.numel(),
-                                               capi.stream_ptr()), 'preference_loss_fwd')
+                                               stream), 'preference_loss_fwd')
     return loss, margin, ws
 
 
-def _preference_bwd(Q, O, logits, ws):
+def _preference_bwd(Q, O, logits, ws, stream):
     dlogits = torch.empty((Q.rows, Q.classes), dtype=logits.dtype, device=logits.device)
     capi.check(lib.edgehip_preference_loss_bwd(byref(Q), byref(O), dlogits.data_ptr(), ws.data_ptr(), ws.numel(),
-                                               capi.stream_ptr()), 'preference_loss_bwd')
+                                               stream), 'preference_loss_bwd')
     return dlogits
 
 
@@ -213,17 +213,23 @@ def preference_loss_grad(logits, taken, seq_ptr, *, ref_logp=None, mask=None, we
     'square': (margin - 1 / (2 beta))^2."""
     Q, O, keep = _preference_args('preference_loss_grad', logits, taken, seq_ptr, ref_logp, mask, weight, beta, label_smoothing,
                                   kind, reduce)
-    with capi.device_of(logits):
-        loss, margin, ws = _preference_fwd(Q, O, logits.device)
-        return PreferenceGrad(loss, margin, _preference_bwd(Q, O, logits, ws))
+    dev = logits.device
+    loss = torch.empty(Q.num_seqs // 2, dtype=torch.float32, device=dev)
+    margin = torch.empty_like(loss)
+    dlogits = torch.empty((Q.rows, Q.classes), dtype=logits.dtype, device=dev)
+    ws = _workspace(Q, dev)
+    with capi.on_device_of(logits) as stream:
+        capi.check(lib.edgehip_preference_loss_grad(byref(Q), byref(O), loss.data_ptr(), margin.data_ptr(), dlogits.data_ptr(),
+                                                    ws.data_ptr(), ws.numel(), stream), 'preference_loss_grad')
+    return PreferenceGrad(loss, margin, dlogits)
 
 
 class _PreferenceLoss(Function):
     @staticmethod
     def forward(ctx, logits, taken, seq_ptr, ref_logp, mask, opts):
         Q, O, keep = _preference_args('preference_loss', logits, taken, seq_ptr, ref_logp, mask, None, **opts)
-        with capi.device_of(logits):
-            loss, margin, ws = _preference_fwd(Q, O, logits.device)
+        with capi.on_device_of(logits) as stream:
+            loss, margin, ws = _preference_fwd(Q, O, logits.device, stream)
         ctx.save_for_backward(logits, taken, seq_ptr, ref_logp, mask, ws)
         ctx.opts = opts
         ctx.mark_non_differentiable(margin)
@@ -234,8 +240,8 @@ class _PreferenceLoss(Function):
         logits, taken, seq_ptr, ref_logp, mask, ws = ctx.saved_tensors
         Q, O, keep = _preference_args('preference_loss', logits, taken, seq_ptr, ref_logp, mask, dloss.float().contiguous(),
                                       **ctx.opts)
-        with capi.device_of(logits):
-            return (_preference_bwd(Q, O, logits, ws),) + (None,) * 5
+        with capi.on_device_of(logits) as stream:
+            return (_preference_bwd(Q, O, logits, ws, stream),) + (None,) * 5
 
 
 def preference_loss(logits, taken, seq_ptr, *, ref_logp=None, mask=None, beta=0.1, label_smoothing=0.0, kind='sigmoid',

@@ -582,7 +582,8 @@ typedef struct edgehip_preference {
     int32_t kind, mean;
 } edgehip_preference;
 /* ws: edgehip_tune_workspace_bytes(Q) bytes, 16-byte aligned.  *_fwd leaves in it what *_bwd (same arguments, weight: the
- * gradients of the losses) needs; policy_loss_grad makes loss and gradient in one pass over the logits.  logp: [rows] or NULL. */
+ * gradients of the losses) needs.  *_grad makes loss and gradient in one call (the policy loss in one pass over the logits; a
+ * preference's gradient needs the sums of all rows first: two).  logp: [rows] or NULL. */
 size_t edgehip_tune_workspace_bytes(const edgehip_logit_rows* Q);
 int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehip_policy* O, float* loss, float* kl, int32_t* clipped,
                             float* logp, void* ws, size_t ws_bytes, void* stream);
@@ -594,6 +595,8 @@ int edgehip_preference_loss_fwd(const edgehip_logit_rows* Q, const edgehip_prefe
                                 size_t ws_bytes, void* stream);
 int edgehip_preference_loss_bwd(const edgehip_logit_rows* Q, const edgehip_preference* O, void* dlogits, void* ws,
                                 size_t ws_bytes, void* stream);
+int edgehip_preference_loss_grad(const edgehip_logit_rows* Q, const edgehip_preference* O, float* loss, float* margin,
+                                 void* dlogits, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- measurement hooks (no counterpart in the reference; used by bench.py's roofline leg) -------
  * When enabled, every kernel launch of the path is bracketed by HIP events on its launch stream.
