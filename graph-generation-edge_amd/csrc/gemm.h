@@ -77,7 +77,7 @@ struct eh_frag3 { eh_u32x4 h[4], m[4], l[4]; };      // [i]: k-group 8i..8i+7 of
 __device__ static inline void eh_split_pair(float x0, float x1, unsigned& ph, unsigned& pm, unsigned& pl) {
     typedef float eh_f2 __attribute__((ext_vector_type(2)));
     const unsigned u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-    // the two remainders of a pair as ONE packed subtraction each (exact either way)
+    // the two remainders of a pair (exact)
     const eh_f2 r = eh_f2{x0, x1} - eh_f2{__uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 & 0xffff0000u)};
     const unsigned v0 = __float_as_uint(r[0]), v1 = __float_as_uint(r[1]);
     const eh_f2 t = r - eh_f2{__uint_as_float(v0 & 0xffff0000u), __uint_as_float(v1 & 0xffff0000u)};
