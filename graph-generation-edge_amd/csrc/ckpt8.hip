@@ -34,26 +34,28 @@ __device__ static inline int ck_exponent(unsigned a) {
     return e < CK_E_MIN ? CK_E_MIN : e > CK_E_MAX ? CK_E_MAX : e;
 }
 
-// log(1 + exp(x)) and its derivative; the larger of 0 and x is split off, so nothing overflows
-__device__ static inline float ck_tanh_softplus(float x) {
-    // tanh(log(1 + e^x)) = ((1 + e^x)^2 - 1) / ((1 + e^x)^2 + 1) = s / (s + 2), s = e^x (e^x + 2); for x > 0 in e^-x:
-    // (1 + 2 w) / (1 + 2 w + 2 w^2)
-    const float w = expf(-fabsf(x));
+// The activations and their derivatives.  FAST, for 16-bit results: e^-|x| and 1 / (1 + .) by the hardware's instructions
+// (together 1e-6 relative, their rounding is 2^-9 or 2^-12); fp32 results take the library's.
+template <bool FAST> __device__ static inline float ck_exp_neg(float x) {       // e^-|x|
+    return FAST ? __builtin_amdgcn_exp2f(fabsf(x) * -1.44269504088896341f) : expf(-fabsf(x));
+}
+template <bool FAST> __device__ static inline float ck_div(float a, float b) { return FAST ? a * __builtin_amdgcn_rcpf(b) : a / b; }
+// tanh(log(1 + e^x)) = ((1 + e^x)^2 - 1) / ((1 + e^x)^2 + 1) = s / (s + 2), s = w (w + 2), w = e^x; for x > 0 in w = e^-x:
+// (1 + 2 w) / (1 + 2 w + 2 w^2)
+template <bool FAST> __device__ static inline float ck_tanh_softplus(float x, float w) {
     const float a = x > 0.0f ? 1.0f + 2.0f * w : w * (w + 2.0f);
     const float b = x > 0.0f ? 2.0f * w * w : 2.0f;
-    return a / (a + b);
+    return ck_div<FAST>(a, a + b);
 }
-__device__ static inline float ck_sigmoid(float x) {
-    const float w = expf(-fabsf(x));
-    return (x >= 0.0f ? 1.0f : w) / (1.0f + w);
+template <bool FAST> __device__ static inline float ck_sigmoid(float x, float w) { return ck_div<FAST>(x >= 0.0f ? 1.0f : w, 1.0f + w); }
+template <bool FAST> __device__ static inline float ck_act(int kind, float x) {
+    const float w = ck_exp_neg<FAST>(x);
+    return x * (kind == EDGEHIP_ACT_SILU ? ck_sigmoid<FAST>(x, w) : ck_tanh_softplus<FAST>(x, w));
 }
-__device__ static inline float ck_act(int kind, float x) {
-    return kind == EDGEHIP_ACT_SILU ? x / (1.0f + expf(-x)) : x * ck_tanh_softplus(x);
-}
-__device__ static inline float ck_dact(int kind, float x) {
-    const float p = ck_sigmoid(x);
+template <bool FAST> __device__ static inline float ck_dact(int kind, float x) {
+    const float w = ck_exp_neg<FAST>(x), p = ck_sigmoid<FAST>(x, w);
     if (kind == EDGEHIP_ACT_SILU) return p * (1.0f + x * (1.0f - p));
-    const float t = ck_tanh_softplus(x);
+    const float t = ck_tanh_softplus<FAST>(x, w);
     return t + x * (1.0f - t * t) * p;
 }
 
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(256) void k_ck_pack(const void* __restrict__ x, int
     if (live && sub == 0) exps[u] = (int8_t)e;
     if (ACT) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ck_act(kind, v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = ck_act<DT != EDGEHIP_F32>(kind, v[i]);
         eh_store8<DT>(y, p.off, p.n, v);
     }
 }
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(256) void k_ck_read(const void* __restrict__ dy, in
     if (BWD) {
         eh_load8<DT>(dy, p.off, p.n, d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = d[i] * ck_dact(kind, v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = d[i] * ck_dact<DT != EDGEHIP_F32>(kind, v[i]);
     }
     eh_store8<DT>(out, p.off, p.n, v);
 }

@@ -23,6 +23,8 @@
 
 // 8-value pieces of its row a thread keeps (64 registers)
 #define TN_KEEP(DT) ((DT) == EDGEHIP_F32 ? 8 : 16)
+// classes up to which a thread takes a row alone
+#define TN_ALONE 32
 #define TN_LOG2E 1.44269504088896341f
 
 struct tn_rows {
@@ -43,7 +45,7 @@ struct tn_rows {
     // per sequence
     const double* scale;                // factor of dterm in the gradient; NULL: weight[s], or each
     const float* weight; double each;
-    double* part;                       // partial sums of the rows' terms (8 classes or less: made with the terms)
+    double* part;                       // partial sums of the rows' terms (TN_ALONE classes or less: made with the terms)
     void* dlogits;                      // dense [R][C]
 };
 
@@ -168,6 +170,14 @@ __device__ static inline float tn_exp(float x) {
     return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
 }
 
+// ln(s) to about 4e-8, s a finite sum of at least 1: the power of two apart, in fp64 (s not finite or 0: as logf has it)
+__device__ static inline double tn_ln(float s) {
+    if (!(s >= 0.5f && s < 3e38f)) return (double)logf(s);
+    const int n = (int)((__float_as_uint(s) - 0x3f3504f3u) >> 23) - (s < 0.70710678f ? 512 : 0);      // s = 2^n f, f in [sqrt(1/2), sqrt(2))
+    const float f = __uint_as_float(__float_as_uint(s) - ((unsigned)n << 23));
+    return (double)n * 0.69314718055994530942 + (double)log1pf(f - 1.0f);
+}
+
 // max and sum over the TPR threads of a row: the running pair of a softmax, merged
 __device__ static inline void tn_merge(float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2);
@@ -222,22 +232,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     const int64_t base = r * T.ld;
     int64_t a = -1;
     const bool counts = r < T.R && tn_counts(T, r, a);
-    constexpr int KEEP = TN_KEEP(DT);
-    eh_raw8<DT> keep[MODE == 2 && TPR > 1 ? KEEP : 1];
+    constexpr int KEEP = MODE != 2 ? 1 : TPR == 1 ? TN_ALONE / 8 : TN_KEEP(DT);
+    eh_raw8<DT> keep[KEEP];
     float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
     float coef = 0.0f;
     const int full = C - 7;                                       // pieces starting below it are whole
-    const bool kept = MODE == 2 && TPR > 1 && C <= TPR * 8 * KEEP;
+    const bool kept = MODE == 2 && C <= TPR * 8 * KEEP;
     if (MODE != 1) {
         if (counts) {
             if (kept) {
 #pragma unroll
-                for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
+                for (int k = 0; k < KEEP; ++k) {
                     const int c = (k * TPR + t) * 8;
                     if (c < full) keep[k].load(reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits) + base + c);
                 }
 #pragma unroll
-                for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
+                for (int k = 0; k < KEEP; ++k) {
                     const int c = (k * TPR + t) * 8;
                     float v[8];
                     if (c < full) { keep[k].get(v); tn_add8<(TPR <= 64)>(m, s, v); }
@@ -259,7 +269,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         if (TPR == 1 && T.old_logp) seq = tn_lane_seq(T, r);
         if (counts) {
             const float xa = (float)reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits)[base + a];
-            logp = (double)xa - (double)m - (TPR > 1 || T.logp64 ? log((double)s) : (double)logf(s));
+            logp = (double)xa - (double)m - tn_ln(s);
             inv = 1.0f / s;
             if (T.old_logp) {
                 if (TPR > 1) seq = tn_seq(T.seq_ptr, T.S, r);
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     if (MODE != 0 && (TPR > 1 || r < T.R)) {
         const float f = -coef * inv;
 #pragma unroll
-        for (int k = 0; k < (MODE == 2 && TPR > 1 ? KEEP : 1); ++k) {
+        for (int k = 0; k < KEEP; ++k) {
             for (int c = (k * TPR + t) * 8; c < C; c += TPR * 8) {
                 float v[8];
                 if (!counts) {
@@ -418,14 +428,22 @@ __global__ __launch_bounds__(256) void k_tn_pref_final(tn_final F) {
 template <int MODE>
 static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
     if (T.R == 0) return EDGEHIP_OK;
-    // threads of a row: as few as can keep it whole, so that a CU has several rows in different phases (8192 x 32003 bf16,
-    // one pass: 1024 threads a row 382 us, 256 BENCH)
+    // Threads of a row: one up to TN_ALONE classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 247 us, one
+    // 36 us), else as few as can keep it whole: what is done once per row is done by all of them, and a CU has rows in
+    // different phases (8192 x 32003 bf16: 1024 threads a row 382 us, 256 242 us; 10^5 x 513 bf16: 64 threads 213 us, 8
+    // 77 us).
     const int per = 8 * (dtype == EDGEHIP_F32 ? TN_KEEP(EDGEHIP_F32) : TN_KEEP(EDGEHIP_BF16));
-    const int tpr = T.C <= 8 ? 1 : T.C <= 512 ? 8 : T.C <= 4096 ? 64 : T.C <= 256 * per ? 256 : 1024;
+    int tpr = 1;
+    if (T.C > TN_ALONE) {
+        tpr = MODE == 1 ? 8 : 4;                                 // (writing only: wider runs of a row pay more)
+        while (tpr < 64 && T.C > tpr * per) tpr *= 2;
+        if (T.C > 64 * per) tpr = 256;
+        while (tpr < 1024 && T.C > tpr * per) tpr *= 2;
+    }
     const int rpb = (tpr < 256 ? 256 : tpr) / tpr;
     const dim3 grid((unsigned)((T.R + rpb - 1) / rpb)), block(tpr < 256 ? 256 : tpr);
 #define TN_TPR(DT, N) case N: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, N, MODE>), grid, block, 0, s, T)); break;
-#define TN_DT(DT) switch (tpr) { TN_TPR(DT, 1) TN_TPR(DT, 8) TN_TPR(DT, 64) TN_TPR(DT, 256) TN_TPR(DT, 1024) }
+#define TN_DT(DT) switch (tpr) { TN_TPR(DT, 1) TN_TPR(DT, 4) TN_TPR(DT, 8) TN_TPR(DT, 16) TN_TPR(DT, 32) TN_TPR(DT, 64) TN_TPR(DT, 256) TN_TPR(DT, 512) TN_TPR(DT, 1024) }
     if (dtype == EDGEHIP_F32) { TN_DT(EDGEHIP_F32) }
     else if (dtype == EDGEHIP_BF16) { TN_DT(EDGEHIP_BF16) }
     else { TN_DT(EDGEHIP_F16) }
@@ -516,7 +534,7 @@ extern "C" int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehi
     hipStream_t s = eh_stream(stream);
     T.logp = logp; T.rowstat = W.stat; T.dterm = W.dterm;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
-    if (T.C > 8) TN_TRY(tn_sum<1>(T, s));                     // (narrower rows: the row kernel makes the partials)
+    if (T.C > TN_ALONE) TN_TRY(tn_sum<1>(T, s));             // (narrower rows: the row kernel makes the partials)
     F.loss = loss; F.kl = kl; F.clipped = clipped;
     EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
@@ -552,7 +570,7 @@ extern "C" int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgeh
     }
     T.logp = logp; T.dlogits = dlogits;
     TN_TRY(tn_launch<2>(Q->dtype, T, s));
-    if (T.C > 8) TN_TRY(tn_sum<1>(T, s));
+    if (T.C > TN_ALONE) TN_TRY(tn_sum<1>(T, s));
     F.scale = nullptr; F.loss = loss; F.kl = kl; F.clipped = clipped;
     EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();

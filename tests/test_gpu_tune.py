@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 TYPES = [F32, BF16, F16]
-CLASSES = [1, 2, 3, 7, 8, 9, 63, 64, 65, 500, 513, 1000, 4096, 4097, 16385, 40001, 65537, 70000]
+CLASSES = [1, 2, 3, 7, 8, 9, 31, 32, 33, 63, 64, 65, 257, 500, 512, 513, 1000, 1025, 2049, 4096, 4097, 8193, 16385, 32769, 40001, 65537, 70000]
 
 
 def step(t):
@@ -145,7 +145,7 @@ def test_policy_classes(classes):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('classes', [2, 50, 700, 5001, 20000])
+@pytest.mark.parametrize('classes', [2, 20, 50, 700, 1500, 5001, 20000, 40000])
 def test_policy_types_and_options(dtype, classes):
     rows = 200 if classes < 1000 else 40
     for k, opt in enumerate((dict(per_row=True), dict(ref=False, kl_coef=0.0), dict(mean=False, weight=torch.tensor([0.5, -1.0, 0.0, 2.0], device='cuda')),
