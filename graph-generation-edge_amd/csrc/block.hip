@@ -11,7 +11,9 @@
 //
 // Bound by HBM: 14 flops a value forward, 26 backward.  Everything between the reads of h, z (dh', dy) and the writes
 // of h', y (dh, dz) stays in registers: a thread owns 8 columns of a row (one 16-byte access of a 16-bit type), the
-// TPR = 2^k threads of a row meet in a wave reduction (and, above 64, in LDS).  The backward pass recomputes u, h' from
+// threads of a row meet in a wave reduction (and, where it has more than 64, in LDS).  16384 x 4096 bf16: forward 104 us,
+// 5.2 TB/s, backward 177 us, 4.5 TB/s (+ 8 us for the partials), against 5.1 TB/s of a large copy; 78208 x 64 fp32 with a
+// gate per graph: 21 us and 32 us (3.8 TB/s), there the start and end of the launches tell.  The backward pass recomputes u, h' from
 // h and z instead of reading a kept h': the same bytes, and the gradient is that of the unrounded h'.  y, too, is made
 // from the unrounded h'.  All statistics and sums are fp32; each output is rounded once.
 //

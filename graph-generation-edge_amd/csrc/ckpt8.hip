@@ -208,17 +208,21 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 // dW[N][K] = dY[M][N]^T X8[M][K], db[n] = sum over m of dY[m][n].
 //
 // The sum runs over the ROWS of both operands, the slow axis of both, while a matrix instruction wants eight consecutive
-// m of one column in a lane.  A thread therefore stages an 8-row x CW-column piece of each operand (16-byte reads of a
-// 16-bit dY), turns it in registers - two rows' values of a column side by side are one v_perm - and writes CW 16-byte
+// m of one column in a lane.  A thread therefore stages 8-row x CW-column pieces of each operand, turns them in registers - two rows' values of a column side by side are one v_perm - and writes CW 16-byte
 // pieces [column][eight m] to LDS.  The piece (m / 8, column c) stands at ((m / 8) T + c') 16 bytes, c' = c with its low
 // three bits xored by the next three: the eight writers of a bank phase, whose columns are 4 or 8 apart, land in eight
 // different slots, and a fragment (32 consecutive columns) still reads 32 consecutive pieces: no bank conflicts.
 //
-// A block owns a T x T tile of dW and a run of rows; four waves, T/2 x T/2 each.  T = 256: 64 (T = 128: 32) bytes are read
-// from LDS per matrix instruction and lane half... the larger tile needs half the LDS reads per flop and is taken where the
-// matrix pipe is the bound.  Two LDS images: while a chunk of BM rows is multiplied, the next one's registers (requested
-// a chunk earlier) are turned and written, and the one after is requested; one barrier a chunk, which waits for LDS
-// only, so that the requests stay in flight across it.
+// A block owns a T x T tile of dW and a run of rows; four waves, T/2 x T/2 each.  T = 256 needs half the LDS reads per flop
+// of T = 128 and is taken where both sides are wider than 128; its 256 accumulators leave one wave a SIMD, so everything
+// else is placed between its matrix instructions: two LDS images, and while a chunk of BM rows is multiplied, the next
+// one's registers (requested a chunk earlier) are turned and written and the one after is requested, in one run of
+// instructions without a branch; one barrier a chunk, which waits for LDS only, so that the requests stay in flight
+// across it.  16384 x 4096 x 4096 bf16: 526 us, 1046 TFLOP/s - the library's bf16 product of that shape, which has no codes
+// to turn, 527 us; the matrix pipe is busy 45 % of the cycles, vector instructions issue in 34 % (at 2.05 GHz).  fp16 /
+// fp32: 573 / 396 TFLOP/s (two / three terms).  78208 x 512 x 128 fp32: 54-60 us, 2.9 TB/s, T = 128 with two blocks a CU.
+// Not kept: a fixed pattern of one matrix instruction and 5 or 6 others (630-670 us); pieces of four rows with wider
+// reads and the exponents group by group (617 us).
 //
 // The rows are split where the tiles alone do not fill the chip; partial tiles go to the workspace and are added in
 // order by k_ck_dw_sum.  db: the block of k-tile j adds up the chunks with number j modulo the k-tiles, so that this work

@@ -221,7 +221,8 @@ __device__ static inline void tn_add8(float& m, float& s, const float (&v)[8]) {
 
 // MODE 0: row statistics (and the policy's per-row terms where T.old_logp is given)
 // MODE 1: the gradient from row statistics;  MODE 2: both at once
-template <int DT, int TPR, int MODE>
+// PIECES: of a row that one thread keeps (8 classes or less: 1)
+template <int DT, int TPR, int MODE, int PIECES = TN_ALONE / 8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
     __shared__ float lds[2 * (TPR < 64 ? 1 : TPR / 64)];
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     const int64_t base = r * T.ld;
     int64_t a = -1;
     const bool counts = r < T.R && tn_counts(T, r, a);
-    constexpr int KEEP = MODE != 2 ? 1 : TPR == 1 ? TN_ALONE / 8 : TN_KEEP(DT);
+    constexpr int KEEP = MODE != 2 ? 1 : TPR == 1 ? PIECES : TN_KEEP(DT);
     eh_raw8<DT> keep[KEEP];
     float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
     float coef = 0.0f;
@@ -443,7 +444,9 @@ static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
     const int rpb = (tpr < 256 ? 256 : tpr) / tpr;
     const dim3 grid((unsigned)((T.R + rpb - 1) / rpb)), block(tpr < 256 ? 256 : tpr);
 #define TN_TPR(DT, N) case N: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, N, MODE>), grid, block, 0, s, T)); break;
-#define TN_DT(DT) switch (tpr) { TN_TPR(DT, 1) TN_TPR(DT, 4) TN_TPR(DT, 8) TN_TPR(DT, 16) TN_TPR(DT, 32) TN_TPR(DT, 64) TN_TPR(DT, 256) TN_TPR(DT, 512) TN_TPR(DT, 1024) }
+#define TN_DT(DT) switch (T.C <= 8 ? 0 : tpr) { \
+        case 0: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, 1, MODE, 1>), grid, block, 0, s, T)); break; \
+        TN_TPR(DT, 1) TN_TPR(DT, 4) TN_TPR(DT, 8) TN_TPR(DT, 16) TN_TPR(DT, 32) TN_TPR(DT, 64) TN_TPR(DT, 256) TN_TPR(DT, 512) TN_TPR(DT, 1024) }
     if (dtype == EDGEHIP_F32) { TN_DT(EDGEHIP_F32) }
     else if (dtype == EDGEHIP_BF16) { TN_DT(EDGEHIP_BF16) }
     else { TN_DT(EDGEHIP_F16) }
