@@ -276,6 +276,10 @@ template <int DT, int CW> struct dw_y {
 #pragma unroll
         for (int i = 0; i < DWORDS; ++i) d[i] = v[i];
     }
+    __device__ inline void clear() {
+#pragma unroll
+        for (int i = 0; i < DWORDS; ++i) d[i] = 0u;
+    }
     __device__ inline float get(int c) const {
         if (DT == EDGEHIP_F32) return __uint_as_float(d[c < DWORDS ? c : 0]);
         const unsigned w = d[c / 2 < DWORDS ? c / 2 : 0];
@@ -339,6 +343,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
             for (int i = 0; i < 8; ++i) {
                 const int64_t r = mu + mb * 8 + i, q = r < m1 ? r : m1 - 1;
                 y[u][i].load(reinterpret_cast<dw_addr>(reinterpret_cast<uint64_t>(dY)) + (q * N + n0 + yc) * ES);
+                if (r >= m1) y[u][i].clear();                    // (an infinity there times step 0 would be NaN)
                 x[u][i] = (unsigned)*reinterpret_cast<const word*>(codes + q * K + kw) >> xs;
                 e[u][i] = r < m1 ? exps[q * KG + (kc >> 6)] : -127;
             }

@@ -115,6 +115,11 @@ class GraphBatch:
         capi.check(capi.lib.edgehip_adj_from_edges(C_byref(self.layout), capi.ptr(ge) if ge.numel() else None,
                                                    ge.shape[0], adj.data_ptr(), capi.stream_ptr()), 'adj_from_edges')
 
+    @property
+    def node_ptr(self):
+        """[B + 1] int32 on the device: the first node of each graph (the `row_ptr` of per-graph operators)."""
+        return self._t['node_ptr']
+
     def new_adj(self):
         return torch.zeros_like(self.adj)
 

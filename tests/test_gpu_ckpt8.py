@@ -252,3 +252,17 @@ def test_other_streams_and_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, both())), k
+
+
+def test_an_infinity_in_the_last_row_and_one_long_row():
+    import edgehip
+    x = torch.rand(45, 64, device='cuda').to(BF16) + 0.5
+    dy = torch.ones(45, 40, device='cuda').to(BF16)
+    dy[44, 7] = float('inf')
+    dw, db = edgehip.ckpt8.linear8_bwd_weight(dy, edgehip.pack8(x))
+    assert bool((dw[7] == float('inf')).all()) and float(db[7]) == float('inf')
+    assert bool(torch.isfinite(dw[torch.arange(40) != 7]).all())
+    long = sample(1, (1 << 20) + 37, F32, seed=9)[0]
+    p = edgehip.pack8(long)
+    codes, exps, value = kept64(long[None])
+    assert p.shape == long.shape and torch.equal(p.exps.cpu().long(), exps) and torch.equal(p.unpack().cpu().double(), value[0])

@@ -194,3 +194,84 @@ def test_tuning_the_graph_sampler_on_its_own_decisions(monkeypatch):
     near(got[1], want[1])
     monkeypatch.setattr(train, '_Ops8', PlainOps8)
     near(got8[1], gradients(True, True)[1])
+
+
+def test_a_gate_per_graph_of_a_batch():
+    """`node_ptr` of a batch is a row_ptr: every graph's nodes see its own row, as graph by graph with one vector."""
+    import edgehip
+    b = H.graph_batch(cases.ragged_graphs(7))
+    p = b.node_ptr.tolist()
+    h, z = torch.randn(b.num_nodes, 64, device='cuda'), torch.randn(b.num_nodes, 64, device='cuda')
+    g, w = torch.randn(b.num_graphs, 64, device='cuda'), torch.ones(64, device='cuda')
+    got = edgehip.gate_norm(h, z, w_pre=w, w_post=w, gate=g, row_ptr=b.node_ptr)
+    for i, (a, c) in enumerate(zip(p, p[1:])):
+        one = edgehip.gate_norm(h[a:c], z[a:c], w_pre=w, w_post=w, gate=g[i])
+        assert torch.equal(one[0], got[0][a:c]) and torch.equal(one[1], got[1][a:c])
+
+
+def _whole(v):
+    """Forward and backward of all operators, through their differentiable forms."""
+    import edgehip
+    leaves = {k: t.detach().requires_grad_(True) for k, t in v.items() if t.is_floating_point() and k not in ('old', 'adv')}
+    h, y = edgehip.gate_norm(leaves['h'], leaves['z'], w_pre=leaves['w'], gate=leaves['g'], kind='rms')
+    x = edgehip.linear8(edgehip.act8(edgehip.linear8(y, leaves['a'])), leaves['b'])
+    a = edgehip.policy_loss(x, v['taken'], v['old'], v['adv'], v['ptr']).loss.sum()
+    b = edgehip.preference_loss(x, v['taken'], v['ptr']).loss.sum()
+    return [a.detach(), b.detach(), h.detach()] + list(torch.autograd.grad(a + b + h.sum(), list(leaves.values())))
+
+
+def _inputs(seed):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device='cuda')
+    return dict(h=n(300, 128), z=n(300, 128), w=n(128), g=n(128), a=n(256, 128) * 0.1, b=n(64, 256) * 0.1,
+                taken=torch.randint(0, 64, (300,), generator=g, device='cuda'), old=n(300) * 0.1 - 4, adv=n(4),
+                ptr=torch.tensor([0, 50, 180, 180, 300], device='cuda'))
+
+
+def test_two_steps_at_once_on_two_streams():
+    v = [_inputs(1), _inputs(2)]
+    want = [_whole(x) for x in v]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    out = [[], []]
+    for k in range(6):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                out[i].append(_whole(v[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for r in out[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_a_whole_step_captured_and_replayed():
+    v = _inputs(3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                          # what a first call sets up is set up outside the graph
+        _whole(v)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _whole(v)
+    for k in range(4):
+        new = _inputs(10 + k)
+        for name in v:
+            v[name].copy_(new[name])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, _whole(v))), k
+
+
+def test_a_second_backward_of_one_forward():
+    import edgehip
+    v = _inputs(4)
+    x = torch.randn(300, 64, device='cuda', requires_grad=True)
+    for loss in (edgehip.policy_loss(x, v['taken'], v['old'], v['adv'], v['ptr']).loss, edgehip.preference_loss(x, v['taken'], v['ptr']).loss):
+        w = torch.arange(1.0, 1 + loss.numel(), device='cuda')
+        (one,) = torch.autograd.grad(loss, x, w, retain_graph=True)
+        (two,) = torch.autograd.grad(loss, x, 2 * w, retain_graph=True)
+        (three,) = torch.autograd.grad(loss, x, w)
+        assert torch.equal(one, three) and bool(((two - 2 * one).abs() <= 1e-6 * one.abs() + 1e-12).all())
