@@ -460,7 +460,7 @@ static int tn_check(const edgehip_logit_rows* Q, bool seqs = true) {
     EH_CHECK_ARG(Q && eh_dtype_ok(Q->dtype) && Q->rows >= 0 && Q->classes >= 1);
     EH_CHECK_ARG(seqs ? Q->seq_ptr && Q->num_seqs >= 1 : (Q->seq_ptr != nullptr) == (Q->num_seqs >= 1) && Q->num_seqs >= 0);
     EH_CHECK_ARG(Q->rows == 0 || (Q->logits && Q->taken && Q->row_stride >= Q->classes));
-    if (Q->rows > (((int64_t)1 << 31) - 1) || Q->num_seqs > (1 << 30)) return EDGEHIP_ERR_TOO_LARGE;
+    if (Q->rows > (((int64_t)1 << 31) - 1) || Q->num_seqs > (1 << 30) || Q->classes > (1 << 30)) return EDGEHIP_ERR_TOO_LARGE;
     return EDGEHIP_OK;
 }
 static tn_rows tn_fill(const edgehip_logit_rows* Q) {

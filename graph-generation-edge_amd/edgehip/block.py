@@ -8,6 +8,7 @@ import ctypes as C
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import capi
 
@@ -72,6 +73,8 @@ def _describe(what, h, z, w_pre, b_pre, w_post, b_post, gate, row_ptr, kind, pre
             capi.same_device(what, 'row_ptr', row_ptr, dev)
             if row_ptr.dtype != torch.int32 or row_ptr.dim() != 1 or not row_ptr.is_contiguous() or row_ptr.numel() < 2:
                 raise ValueError(f'{what}: row_ptr must be a dense int32 vector of groups + 1 offsets')
+            if row_ptr.numel() > 65536:
+                raise ValueError(f'{what}: up to 65535 groups, got {row_ptr.numel() - 1}')
             G.groups = row_ptr.numel() - 1
             if gate.shape != (G.groups, dim):
                 raise ValueError(f'{what}: a gate per group must be [{G.groups}, {dim}], got {tuple(gate.shape)}')
@@ -104,7 +107,8 @@ def gate_norm_fwd(h, z, *, w_pre=None, b_pre=None, w_post=None, b_post=None, gat
     """(h', y, stats): h' = res_scale h + gate N_post(z), y = N_pre(h').  Not differentiable by itself.
 
     h, z: [..., dim], z fp32 / bf16 / fp16, h of the same type or fp32 (h' like h, y like z).  gate: None, [dim], one row
-    per group of rows [groups, dim] with row_ptr [groups + 1] int32 (a batch's node_ptr), or one per row, shaped like h.
+    per group of rows [groups, dim] (65535 groups at most) with row_ptr [groups + 1] int32 (a batch's node_ptr), or one per
+    row, shaped like h.
     w_*, b_*: [dim], fp32 or of z's type; None: ones / zeros.  post=False: z itself is gated; pre=False: y is None.
     stats [rows, 4] (want_stats) is what `gate_norm_bwd` needs besides h and z."""
     G, h, z, gate = _describe('gate_norm', h, z, w_pre, b_pre, w_post, b_post, gate, row_ptr, kind, pre, post, res_scale, eps)
@@ -167,6 +171,7 @@ class _GateNorm(Function):
         return h_out, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh_out, dy):
         h, z, w_pre, b_pre, w_post, b_post, gate, row_ptr, stats = ctx.saved_tensors
         G, h, z, gate = _describe('gate_norm', h, z, w_pre, b_pre, w_post, b_post, gate, row_ptr, **ctx.opts)

@@ -6,6 +6,7 @@ of: 1 + 1/64 bytes a value, off by at most 1/127 of the largest value of the gro
 are those of the exact input, only the gradients (of the activation's input, of the weight) read the kept values."""
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import capi
 
@@ -128,15 +129,15 @@ def linear8_bwd_weight(dy, kept, bias=True):
     code = _against(what, dy, kept)
     if dy.dim() < 1 or dy.shape[:-1] != kept.shape[:-1] or dy.shape[-1] < 1:
         raise ValueError(f'{what}: dy must be {list(kept.shape[:-1])} x [outputs], got {tuple(dy.shape)}')
+    n, k = dy.shape[-1], kept.shape[-1]
+    if max(n, k) > 1 << 22:
+        raise ValueError(f'{what}: layers of up to {1 << 22} inputs and outputs, got {k} and {n}')
     capi.on_gpu(what, dy)
     dy = dy.contiguous()
-    n, k = dy.shape[-1], kept.shape[-1]
     m = dy.numel() // n
     dw = torch.empty((n, k), dtype=torch.float32, device=dy.device)
     db = torch.empty(n, dtype=torch.float32, device=dy.device) if bias else None
     nbytes = lib.edgehip_linear8_workspace_bytes(code, m, n, k)
-    if nbytes == 0:
-        raise ValueError(f'{what}: layers of up to {1 << 22} inputs and outputs')
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
     with capi.on_device_of(dy) as stream:
         capi.check(lib.edgehip_linear8_bwd_weight(code, dy.data_ptr(), kept.codes.data_ptr(), kept.exps.data_ptr(), m, n, k,
@@ -153,6 +154,7 @@ class _Act8(Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dtype, kind = ctx.kept
         return act8_bwd(dy, Packed8(*ctx.saved_tensors, dtype), kind), None
@@ -171,6 +173,12 @@ def _own_products(x, w):
     return x.dtype == torch.float32 and x.dim() == 2 and k % 64 == 0 and n % 64 == 0
 
 
+def _aligned(t):
+    """t as the package's products read it: dense, from a 16-byte boundary."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
 class _Linear8(Function):
     @staticmethod
     def forward(ctx, x, w, b, kept):
@@ -179,18 +187,19 @@ class _Linear8(Function):
         if ctx.own:
             y = torch.empty((x.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)
             if x.shape[0]:
-                wc = w.contiguous()
+                xc, wc, bc = _aligned(x), _aligned(w), None if b is None else _aligned(b)
                 with capi.on_device_of(x) as stream:
-                    capi.check(lib.edgehip_linear_fwd(x.data_ptr(), x.shape[0], w.shape[1], wc.data_ptr(),
-                                                      capi.ptr(b.contiguous() if b is not None else None), w.shape[0], 0,
-                                                      y.data_ptr(), stream), 'linear_fwd')
+                    capi.check(lib.edgehip_linear_fwd(xc.data_ptr(), x.shape[0], w.shape[1], wc.data_ptr(), capi.ptr(bc),
+                                                      w.shape[0], 0, y.data_ptr(), stream), 'linear_fwd')
         else:
-            y = torch.nn.functional.linear(x, w, b)
+            with torch.autocast(x.device.type, enabled=False):   # y is of x's type, whatever surrounds the call
+                y = torch.nn.functional.linear(x, w, b)
         ctx.save_for_backward(w, kept and kept.codes, kept and kept.exps)
         ctx.has_bias, ctx.dtype = b is not None, x.dtype
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         w, codes, exps = ctx.saved_tensors
         dy = dy.contiguous()
@@ -201,19 +210,22 @@ class _Linear8(Function):
                 dx = torch.empty((dy.shape[0], k), dtype=dy.dtype, device=dy.device)
                 if dy.shape[0]:
                     wt = torch.empty(k * n, dtype=torch.float32, device=dy.device)
-                    wc = w.contiguous()
+                    yc, wc = _aligned(dy), _aligned(w)
                     with capi.on_device_of(dy) as stream:
-                        capi.check(lib.edgehip_linear_bwd_input(dy.data_ptr(), dy.shape[0], n, wc.data_ptr(), k, wt.data_ptr(),
+                        capi.check(lib.edgehip_linear_bwd_input(yc.data_ptr(), dy.shape[0], n, wc.data_ptr(), k, wt.data_ptr(),
                                                                 dx.data_ptr(), stream), 'linear_bwd_input')
             else:
-                dx = torch.matmul(dy, w)
+                with torch.autocast(dy.device.type, enabled=False):
+                    dx = torch.matmul(dy, w)
         want_db = ctx.has_bias and ctx.needs_input_grad[2]
         if ctx.needs_input_grad[1]:
             dw, db = linear8_bwd_weight(dy, Packed8(codes, exps, ctx.dtype), bias=want_db)
             dw = dw.to(w.dtype)
             db = db.to(w.dtype) if want_db else None
         elif want_db:
-            db = dy.float().reshape(-1, dy.shape[-1]).sum(0).to(w.dtype)
+            # (no library sum: a captured one can hold a memory-set node; the checkpoint of an input of one zero is a stand-in)
+            none = torch.zeros(dy.shape[:-1] + (1,), dtype=torch.int8, device=dy.device)
+            db = linear8_bwd_weight(dy, Packed8(none, none.reshape(-1, 1), ctx.dtype))[1].to(w.dtype)
         return dx, dw, db, None
 
 
@@ -230,6 +242,8 @@ def linear8(x, w, b=None, kept=None):
             capi.same_device('linear8', name, t, x.device)
     if kept is not None and (not isinstance(kept, Packed8) or kept.shape != x.shape):
         raise ValueError('linear8: kept must be pack8(x)')
+    if kept is not None:
+        capi.same_device('linear8', 'kept', kept.codes, x.device)
     if not (torch.is_grad_enabled() and w.requires_grad):
         kept = None
     elif kept is None:

@@ -14,6 +14,7 @@ from collections import namedtuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import capi
 
@@ -43,6 +44,8 @@ def _describe(what, logits, taken, seq_ptr, mask):
         raise ValueError(f'{what}: logits must be [rows, classes], got {tuple(logits.shape)}')
     code = capi.dtype_code(what, 'logits', logits)
     rows, classes = logits.shape
+    if max(classes, 0 if seq_ptr is None else seq_ptr.numel() - 1) > 1 << 30:
+        raise ValueError(f'{what}: up to 2^30 classes and sequences')
     dev = logits.device
     if classes > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < classes:
         logits = logits.contiguous()
@@ -152,6 +155,7 @@ class _PolicyLoss(Function):
         return loss, kl, clipped, logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, *_):
         logits, taken, old_logp, advantage, seq_ptr, ref_logp, mask, ws = ctx.saved_tensors
         Q, O, keep = _policy_args('policy_loss', logits, taken, old_logp, advantage, seq_ptr, ref_logp, mask,
@@ -236,6 +240,7 @@ class _PreferenceLoss(Function):
         return loss, margin
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, _):
         logits, taken, seq_ptr, ref_logp, mask, ws = ctx.saved_tensors
         Q, O, keep = _preference_args('preference_loss', logits, taken, seq_ptr, ref_logp, mask, dloss.float().contiguous(),

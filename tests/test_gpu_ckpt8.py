@@ -266,3 +266,60 @@ def test_an_infinity_in_the_last_row_and_one_long_row():
     p = edgehip.pack8(long)
     codes, exps, value = kept64(long[None])
     assert p.shape == long.shape and torch.equal(p.exps.cpu().long(), exps) and torch.equal(p.unpack().cpu().double(), value[0])
+
+
+def test_a_layer_whose_weight_is_fixed_captured():
+    """Only the bias learns: its gradient, replayed with eager work between, is the eager one each time."""
+    import edgehip
+    x, dy = torch.randn(40000, 96, device='cuda').to(BF16), torch.randn(40000, 200, device='cuda').to(BF16)
+    w, b = torch.randn(200, 96, device='cuda').to(BF16), torch.zeros(200, device='cuda').to(BF16)
+
+    def run():
+        leaf = b.detach().requires_grad_(True)
+        return torch.autograd.grad(edgehip.linear8(x, w, leaf), leaf, dy)[0]
+    run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(4):
+        dy.copy_(torch.randn(dy.shape, device='cuda') * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, run()), k
+        want = dy.double().sum(0)
+        # fp32 sums in two levels of a few hundred terms each, one rounding to bf16
+        assert bool(((out.double() - want).abs() <= step(BF16) * want.abs() + 1000 * U * dy.double().abs().sum(0)).all()), k
+
+
+@pytest.mark.parametrize('shift', [0, 1, 2, 3])
+def test_a_layer_on_views_that_start_anywhere(shift):
+    import edgehip
+    m, n, k = 70, 64, 128
+
+    def view(r, c, seed):
+        flat = torch.randn(r * c + 4, generator=torch.Generator(device='cuda').manual_seed(seed), device='cuda')
+        return flat[shift:shift + r * c].view(r, c)
+    x, w, dy, b = view(m, k, 1), view(n, k, 2), view(m, n, 3), view(1, n, 4)[0]
+    got, want = [], []
+    for out, form in ((got, lambda t: t), (want, lambda t: t.clone())):
+        leaves = [form(t).detach().requires_grad_(True) for t in (x, w, b)]
+        y = edgehip.linear8(*leaves)
+        out += [y.detach()] + list(torch.autograd.grad(y, leaves, form(dy)))
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_a_layer_keeps_its_type_inside_autocast():
+    import edgehip
+    x = torch.randn(33, 50, device='cuda').requires_grad_(True)
+    w = torch.randn(30, 50, device='cuda').requires_grad_(True)
+    y = edgehip.linear8(x, w)
+    with torch.autocast('cuda', dtype=BF16):
+        z = edgehip.linear8(x, w)
+        grads = torch.autograd.grad(z, [x, w], torch.ones_like(z))
+    assert z.dtype == F32 and torch.equal(y, z)
+    assert all(torch.equal(a, c) for a, c in zip(grads, torch.autograd.grad(y, [x, w], torch.ones_like(y))))

@@ -275,3 +275,18 @@ def test_a_second_backward_of_one_forward():
         (two,) = torch.autograd.grad(loss, x, 2 * w, retain_graph=True)
         (three,) = torch.autograd.grad(loss, x, w)
         assert torch.equal(one, three) and bool(((two - 2 * one).abs() <= 1e-6 * one.abs() + 1e-12).all())
+
+
+def test_second_derivatives_are_refused():
+    """The backward passes are kernels without a graph of their own: a gradient of a gradient is an error, not a wrong value."""
+    import edgehip
+    v = lambda *s: torch.randn(*s, device='cuda').requires_grad_(True)
+    ptr = torch.tensor([0, 3, 8], device='cuda')
+    taken = torch.zeros(8, dtype=torch.int64, device='cuda')
+    x, z, w = v(8, 64), v(8, 64), v(64, 64)
+    for out in (edgehip.gate_norm(x, z)[1], edgehip.act8(x), edgehip.linear8(x, w),
+                edgehip.policy_loss(x, taken, torch.zeros(8, device='cuda'), torch.ones(2, device='cuda'), ptr).loss,
+                edgehip.preference_loss(x, taken, ptr).loss):
+        first, = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            first.sum().backward()

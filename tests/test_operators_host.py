@@ -182,3 +182,18 @@ def test_tune_c_refusals():
     assert pf(rows(), R(beta=0.0)) == capi.ERR_ARG and pf(rows(), R(kind=2)) == capi.ERR_ARG and pf(rows(), R(label_smoothing=0.6)) == capi.ERR_ARG
     assert pf(rows(num_seqs=3), R(), nb=1 << 20) == capi.ERR_ARG and pf(rows(), R(), nb=need - 1) == capi.ERR_WORKSPACE
     assert L.edgehip_row_logp(rows(num_seqs=0), p, None) == capi.ERR_ARG and L.edgehip_row_logp(rows(), None, None) == capi.ERR_ARG
+
+
+def test_sizes_that_would_not_fit_their_field():
+    """Wider than 32 bits: refused, never cut off.  (Expanded views: nothing of that size is allocated.)"""
+    import edgehip
+    from edgehip import capi, ckpt8
+    wide = vec(1, 1).expand(1, (1 << 32) + 5)
+    with pytest.raises(ValueError, match='2\\^30 classes'):
+        edgehip.row_logp(wide, i64(0))
+    with pytest.raises(ValueError, match='inputs and outputs'):
+        ckpt8.linear8_bwd_weight(wide, ckpt8.Packed8(vec(1, 64, t=torch.int8), vec(1, 1, t=torch.int8), torch.float32))
+    with pytest.raises(ValueError, match='65535 groups'):
+        edgehip.gate_norm(H, Z, gate=vec(65536, 8), row_ptr=torch.zeros(65537, dtype=torch.int32))
+    Q = capi.LogitRows(rows=1, row_stride=(1 << 30) + 1, classes=(1 << 30) + 1, num_seqs=1, logits=4096, taken=4096, seq_ptr=4096)
+    assert capi.lib.edgehip_row_logp(byref(Q), ctypes.c_void_p(4096), None) == capi.ERR_TOO_LARGE
