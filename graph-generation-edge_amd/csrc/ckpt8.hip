@@ -21,6 +21,7 @@
 
 typedef float ck_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 ck_bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int ck_u32u __attribute__((aligned(1)));
 typedef unsigned int ck_u32x4 __attribute__((ext_vector_type(4)));
 
 // step of a group, or NaN
@@ -69,16 +70,20 @@ __device__ static inline ck_place ck_locate(unsigned u, unsigned KG, int K, int 
     return ck_place{(int64_t)row * K + c, K - c};
 }
 
-template <int DT, bool ACT>
+template <int DT, bool ACT, bool TINY>
 __global__ __launch_bounds__(256) void k_ck_pack(const void* __restrict__ x, int kind, void* __restrict__ y, int8_t* __restrict__ codes,
-                                                 int8_t* __restrict__ exps, unsigned ngroups, unsigned KG, int K) {
+                                                 int8_t* __restrict__ exps, unsigned ngroups, unsigned KG, int K, int64_t end) {
     const unsigned u = blockIdx.x * 32u + (threadIdx.x >> 3);
     const int sub = threadIdx.x & 7;
     const bool live = u < ngroups;
     ck_place p = ck_locate(live ? u : 0, KG, K, sub);
     if (!live) p.n = 0;
+    const eh_at at = eh_place(p.off, p.n, end);
+    eh_raw8<DT> in;
     float v[8];
-    eh_load8<DT>(x, p.off, p.n, v);
+    eh_get<DT, TINY>(in, x, at);
+    in.get(v);
+    eh_own<TINY>(v, at.n, at.back);
     unsigned a = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -98,12 +103,15 @@ __global__ __launch_bounds__(256) void k_ck_pack(const void* __restrict__ x, int
         const int q = e == CK_E_BAD ? 0 : (int)fminf(fmaxf(rintf(v[i] * down), -127.0f), 127.0f);    // exact product
         w[i >> 2] |= ((unsigned)q & 0xffu) << (8 * (i & 3));
     }
+    int8_t* q = codes + p.off;
     if (p.n >= 8) {
-        *reinterpret_cast<eh_u32x2u*>(codes + p.off) = eh_u32x2u{w[0], w[1]};
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < p.n) codes[p.off + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
+        *reinterpret_cast<eh_u32x2u*>(q) = eh_u32x2u{w[0], w[1]};
+    } else if (p.n > 0) {                                        // in pieces of four, two and one
+        if (p.n & 4) *reinterpret_cast<ck_u32u*>(q) = w[0];
+        const unsigned rest = p.n & 4 ? w[1] : w[0];
+        q += p.n & 4;
+        if (p.n & 2) { q[0] = (int8_t)rest; q[1] = (int8_t)(rest >> 8); }
+        if (p.n & 1) q[p.n & 2] = (int8_t)(p.n & 2 ? rest >> 16 : rest);
     }
     if (live && sub == 0) exps[u] = (int8_t)e;
     if (ACT) {
@@ -113,29 +121,36 @@ __global__ __launch_bounds__(256) void k_ck_pack(const void* __restrict__ x, int
     }
 }
 
-__device__ static inline void ck_load_codes(const int8_t* codes, int64_t off, int n, float step, float (&o)[8]) {
-    if (n >= 8) {
-        const eh_u32x2u w = *reinterpret_cast<const eh_u32x2u*>(codes + off);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * step;
+// eight codes where eh_place puts them, as values; what lies behind a row's end stays what it is
+template <bool TINY>
+__device__ static inline void ck_load_codes(const int8_t* codes, const eh_at& at, float step, float (&o)[8]) {
+    uint64_t w = 0;
+    if (!TINY) {
+        const eh_u32x2u v = *reinterpret_cast<const eh_u32x2u*>(codes + at.off);
+        w = ((uint64_t)v[1] << 32 | v[0]) >> (8 * at.back);
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = i < n ? (float)codes[off + i] * step : 0.0f;
+        for (int i = 0; i < at.n; ++i) w |= (uint64_t)(uint8_t)codes[at.off + at.back + i] << (8 * i);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)(int8_t)(w >> (8 * i)) * step;
 }
 
 // BWD: dx = dy act'(kept x); else out = kept x
-template <int DT, bool BWD>
+template <int DT, bool BWD, bool TINY>
 __global__ __launch_bounds__(256) void k_ck_read(const void* __restrict__ dy, int kind, const int8_t* __restrict__ codes,
                                                  const int8_t* __restrict__ exps, void* __restrict__ out, unsigned ngroups, unsigned KG,
-                                                 int K) {
+                                                 int K, int64_t end) {
     const unsigned u = blockIdx.x * 32u + (threadIdx.x >> 3);
     if (u >= ngroups) return;
     const ck_place p = ck_locate(u, KG, K, threadIdx.x & 7);
+    const eh_at at = eh_place(p.off, p.n, end);
+    eh_raw8<DT> in;
     float v[8], d[8];
-    ck_load_codes(codes, p.off, p.n, ck_step(exps[u]), v);
+    if (BWD) eh_get<DT, TINY>(in, dy, at);
+    ck_load_codes<TINY>(codes, at, ck_step(exps[u]), v);
     if (BWD) {
-        eh_load8<DT>(dy, p.off, p.n, d);
+        in.get(d);
+        eh_own<TINY>(d, at.n, at.back);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = d[i] * ck_dact<DT != EDGEHIP_F32>(kind, v[i]);
     }
@@ -162,11 +177,13 @@ static int ck_pack(int dtype, const void* x, int kind, void* y, int64_t M, int64
     EH_CHECK_ARG(x && codes && exps && (!ACT || y));
     hipStream_t s = eh_stream(stream);
     const dim3 grid((ng + 31) / 32), block(256);
-#define CK_GO(DT) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_pack<DT, ACT>), grid, block, 0, s, x, kind, y, codes, exps, ng, KG, (int)K))
+#define CK_AS(DT, TINY) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_pack<DT, ACT, TINY>), grid, block, 0, s, x, kind, y, codes, exps, ng, KG, (int)K, M * K))
+#define CK_GO(DT) do { if (M * K < 8) CK_AS(DT, true); else CK_AS(DT, false); } while (0)
     if (dtype == EDGEHIP_F32) CK_GO(EDGEHIP_F32);
     else if (dtype == EDGEHIP_BF16) CK_GO(EDGEHIP_BF16);
     else CK_GO(EDGEHIP_F16);
 #undef CK_GO
+#undef CK_AS
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -180,11 +197,13 @@ static int ck_read(int dtype, const void* dy, int kind, int64_t M, int64_t K, co
     EH_CHECK_ARG(codes && exps && out && (!BWD || dy));
     hipStream_t s = eh_stream(stream);
     const dim3 grid((ng + 31) / 32), block(256);
-#define CK_GO(DT) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_read<DT, BWD>), grid, block, 0, s, dy, kind, codes, exps, out, ng, KG, (int)K))
+#define CK_AS(DT, TINY) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_read<DT, BWD, TINY>), grid, block, 0, s, dy, kind, codes, exps, out, ng, KG, (int)K, M * K))
+#define CK_GO(DT) do { if (M * K < 8) CK_AS(DT, true); else CK_AS(DT, false); } while (0)
     if (dtype == EDGEHIP_F32) CK_GO(EDGEHIP_F32);
     else if (dtype == EDGEHIP_BF16) CK_GO(EDGEHIP_BF16);
     else CK_GO(EDGEHIP_F16);
 #undef CK_GO
+#undef CK_AS
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
