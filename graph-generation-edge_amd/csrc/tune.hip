@@ -64,6 +64,18 @@ __device__ static inline int tn_seq(const int64_t* __restrict__ ptr, int S, int6
     return lo;
 }
 
+// the same in a wave of up to RPW consecutive rows, r counted: searched once, by the scalar unit, where they all lie in the
+// sequence of the first
+__device__ static inline int64_t tn_first(int64_t r) {
+    return ((int64_t)__builtin_amdgcn_readfirstlane((int)(r >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)r);
+}
+template <int RPW>
+__device__ static inline int tn_wave_seq(const int64_t* __restrict__ ptr, int S, int64_t r) {
+    const int64_t first = tn_first(r);
+    const int g = tn_seq(ptr, S, first);
+    return RPW == 1 || first + RPW - 1 < ptr[g + 1] ? g : tn_seq(ptr, S, r);
+}
+
 __device__ static inline double tn_scale(const tn_rows& T, int seq) {
     return T.scale ? T.scale[seq] : T.weight ? (double)T.weight[seq] : T.each;
 }
@@ -109,7 +121,7 @@ __device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, d
 // The sequence of this lane's row r (64 consecutive rows a wave), -1 where it lies in none.  Where the wave's first and last
 // row lie in one sequence - most waves - the search is done once, by the scalar unit.
 __device__ static inline int tn_lane_seq(const tn_rows& T, int64_t r) {
-    const int64_t first = ((int64_t)__builtin_amdgcn_readfirstlane((int)(r >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)r);
+    const int64_t first = tn_first(r);
     if (first >= T.seq_ptr[0] && first < T.seq_ptr[T.S]) {
         const int g = tn_seq(T.seq_ptr, T.S, first);
         if (first + 63 < T.seq_ptr[g + 1] && first + 63 < T.R) return g;
@@ -225,6 +237,7 @@ __device__ static inline void tn_add8(float& m, float& s, const float (&v)[8]) {
 template <int DT, int TPR, int MODE, int PIECES = TN_ALONE / 8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
+    constexpr int RPW = TPR < 64 ? 64 / TPR : 1;
     __shared__ float lds[2 * (TPR < 64 ? 1 : TPR / 64)];
     const int t = threadIdx.x % TPR;
     const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -237,28 +250,40 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     eh_raw8<DT> keep[KEEP];
     float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
     float coef = 0.0f;
-    const int full = C - 7;                                       // pieces starting below it are whole
-    const bool kept = MODE == 2 && C <= TPR * 8 * KEEP;
+    // Pieces of eight values, all whole: the last one of a row ends with it and begins inside the one before, those values are
+    // left out of the sum and their gradient is written twice, to the same bits.  (8 classes or less: one piece, value by value.)
+    constexpr bool WHOLE = TPR > 1 || PIECES > 1;
+    const typename eh_elem<DT>::type* const row = reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits) + base;
+    auto start = [&](int c) { return WHOLE && c > C - 8 ? C - 8 : c; };
+    auto add = [&](float (&v)[8], int c) {
+        if (WHOLE && c > C - 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < c - (C - 8) ? -__builtin_inff() : v[i];
+        }
+        tn_add8<(TPR <= 64)>(m, s, v);
+    };
+    const bool kept = MODE == 2 && WHOLE && C <= TPR * 8 * KEEP;
     if (MODE != 1) {
         if (counts) {
             if (kept) {
 #pragma unroll
                 for (int k = 0; k < KEEP; ++k) {
-                    const int c = (k * TPR + t) * 8;
-                    if (c < full) keep[k].load(reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits) + base + c);
+                    if (k * TPR * 8 >= C) break;
+                    keep[k].load(row + start((k * TPR + t) * 8));
                 }
 #pragma unroll
                 for (int k = 0; k < KEEP; ++k) {
+                    if (k * TPR * 8 >= C) break;
                     const int c = (k * TPR + t) * 8;
                     float v[8];
-                    if (c < full) { keep[k].get(v); tn_add8<(TPR <= 64)>(m, s, v); }
-                    else if (c < C) { eh_load8<DT>(T.logits, base + c, C - c, v, -__builtin_inff()); tn_add8<(TPR <= 64)>(m, s, v); }
+                    keep[k].get(v);
+                    if (c < C) add(v, c);
                 }
             } else {
                 for (int c = t * 8; c < C; c += TPR * 8) {
                     float v[8];
-                    eh_load8<DT>(T.logits, base + c, C - c, v, -__builtin_inff());
-                    tn_add8<(TPR <= 64)>(m, s, v);
+                    eh_load8<DT>(row, start(c), WHOLE ? 8 : C, v, -__builtin_inff());
+                    add(v, c);
                 }
             }
             tn_row_merge<TPR>(m, s, lds);                         // (a row counts for all of its threads or none)
@@ -269,11 +294,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         int seq = -1;
         if (TPR == 1 && T.old_logp) seq = tn_lane_seq(T, r);
         if (counts) {
-            const float xa = (float)reinterpret_cast<const typename eh_elem<DT>::type*>(T.logits)[base + a];
+            const float xa = (float)row[a];
             logp = (double)xa - (double)m - tn_ln(s);
             inv = 1.0f / s;
             if (T.old_logp) {
-                if (TPR > 1) seq = tn_seq(T.seq_ptr, T.S, r);
+                if (TPR > 1) seq = tn_wave_seq<RPW>(T.seq_ptr, T.S, r);
                 d = tn_policy(T, r, seq, logp, term, kl, cut);
                 if (MODE == 2) coef = (float)((double)d * tn_scale(T, seq));
             }
@@ -297,21 +322,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     } else if (counts) {
         m = T.rowstat[2 * r];
         inv = T.rowstat[2 * r + 1];
-        const int seq = tn_seq(T.seq_ptr, T.S, r);
+        const int seq = tn_wave_seq<RPW>(T.seq_ptr, T.S, r);
         coef = (float)(T.dterm ? (double)T.dterm[r] * tn_scale(T, seq) : tn_scale(T, seq));
     }
     if (MODE != 0 && (TPR > 1 || r < T.R)) {
         const float f = -coef * inv;
 #pragma unroll
         for (int k = 0; k < KEEP; ++k) {
-            for (int c = (k * TPR + t) * 8; c < C; c += TPR * 8) {
+            if (k * TPR * 8 >= C) break;
+            for (int from = (k * TPR + t) * 8; from < C; from += TPR * 8) {
+                const int c = start(from);
                 float v[8];
                 if (!counts) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
                 } else {
-                    if (kept && c < full) keep[k].get(v);
-                    else eh_load8<DT>(T.logits, base + c, C - c, v, 0.0f);
+                    if (kept) keep[k].get(v);
+                    else eh_load8<DT>(row, c, WHOLE ? 8 : C, v);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = f * __builtin_amdgcn_exp2f((v[i] - m) * TN_LOG2E);
                     if (a >= c && a < c + 8) {
@@ -319,7 +346,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
                         for (int i = 0; i < 8; ++i) if (a == c + i) v[i] += coef;
                     }
                 }
-                eh_store8<DT>(T.dlogits, r * C + c, C - c, v);
+                eh_store8<DT>(T.dlogits, r * C + c, WHOLE ? 8 : C, v);
                 if (kept) break;
             }
             if (!kept) break;
