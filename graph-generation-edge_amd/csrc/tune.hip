@@ -23,8 +23,10 @@
 
 // 8-value pieces of its row a thread keeps (64 registers)
 #define TN_KEEP(DT) ((DT) == EDGEHIP_F32 ? 8 : 16)
-// classes up to which a thread takes a row alone
-#define TN_ALONE 32
+// Classes up to which a thread takes a row alone.  Rows that are read once and kept: 128 bytes (10^6 x 33 / 10^6 x 48 bf16,
+// policy loss and gradient: four threads a row 105 / 102 us, one 62 / 70 us; 10^6 x 48 fp32: 128 us, 147 us).  Only written
+// (preference loss and gradient, 10^6 x 24 / 10^6 x 32 bf16: one 71 / 100 us, four 60 / 64 us): 16 classes.
+#define TN_ALONE(DT, MODE) ((MODE) == 1 ? 16 : (DT) != EDGEHIP_F32 ? 64 : 32)
 #define TN_LOG2E 1.44269504088896341f
 
 struct tn_rows {
@@ -45,7 +47,7 @@ struct tn_rows {
     // per sequence
     const double* scale;                // factor of dterm in the gradient; NULL: weight[s], or each
     const float* weight; double each;
-    double* part;                       // partial sums of the rows' terms (TN_ALONE classes or less: made with the terms)
+    double* part;                       // partial sums of the rows' terms (rows a thread takes alone: made with the terms)
     void* dlogits;                      // dense [R][C]
 };
 
@@ -234,7 +236,7 @@ __device__ static inline void tn_add8(float& m, float& s, const float (&v)[8]) {
 // MODE 0: row statistics (and the policy's per-row terms where T.old_logp is given)
 // MODE 1: the gradient from row statistics;  MODE 2: both at once
 // PIECES: of a row that one thread keeps (8 classes or less: 1)
-template <int DT, int TPR, int MODE, int PIECES = TN_ALONE / 8>
+template <int DT, int TPR, int MODE, int PIECES = 4>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
     constexpr int RPW = TPR < 64 ? 64 / TPR : 1;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     const int64_t base = r * T.ld;
     int64_t a = -1;
     const bool counts = r < T.R && tn_counts(T, r, a);
-    constexpr int KEEP = MODE != 2 ? 1 : TPR == 1 ? PIECES : TN_KEEP(DT);
+    constexpr int KEEP = MODE == 1 ? 1 : TPR == 1 ? PIECES : MODE == 2 ? TN_KEEP(DT) : 1;
     eh_raw8<DT> keep[KEEP];
     float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
     float coef = 0.0f;
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         }
         tn_add8<(TPR <= 64)>(m, s, v);
     };
-    const bool kept = MODE == 2 && WHOLE && C <= TPR * 8 * KEEP;
+    const bool kept = MODE != 1 && WHOLE && C <= TPR * 8 * KEEP;
     if (MODE != 1) {
         if (counts) {
             if (kept) {
@@ -453,32 +455,49 @@ __global__ __launch_bounds__(256) void k_tn_pref_final(tn_final F) {
 }
 
 // ---- entry points -------------------------------------------------------------------------------------------------
+template <int DT, int MODE>
+static void tn_go(const tn_rows& T, int tpr, dim3 grid, dim3 block, hipStream_t s) {
+#define TN_RUN(...) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<__VA_ARGS__>), grid, block, 0, s, T))
+    if (T.C <= 8) { TN_RUN(DT, 1, MODE, 1); return; }
+    if constexpr (TN_ALONE(DT, MODE) > 32) {
+        if (tpr == 1 && T.C > 32) { TN_RUN(DT, 1, MODE, 8); return; }
+    }
+    switch (tpr) {
+        case 1: TN_RUN(DT, 1, MODE); break;
+        case 4: TN_RUN(DT, 4, MODE); break;
+        case 8: TN_RUN(DT, 8, MODE); break;
+        case 16: TN_RUN(DT, 16, MODE); break;
+        case 32: TN_RUN(DT, 32, MODE); break;
+        case 64: TN_RUN(DT, 64, MODE); break;
+        case 256: TN_RUN(DT, 256, MODE); break;
+        case 512: TN_RUN(DT, 512, MODE); break;
+        default: TN_RUN(DT, 1024, MODE);
+    }
+#undef TN_RUN
+}
+template <int MODE> static int tn_alone(int dtype) { return dtype == EDGEHIP_F32 ? TN_ALONE(EDGEHIP_F32, MODE) : TN_ALONE(EDGEHIP_BF16, MODE); }
 template <int MODE>
 static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
     if (T.R == 0) return EDGEHIP_OK;
-    // Threads of a row: one up to TN_ALONE classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 247 us, one
+    // Threads of a row: one for few classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 247 us, one
     // 36 us), else as few as can keep it whole: what is done once per row is done by all of them, and a CU has rows in
-    // different phases (8192 x 32003 bf16: 1024 threads a row 382 us, 256 242 us; 10^5 x 513 bf16: 64 threads 213 us, 8
-    // 77 us).
+    // different phases (8192 x 32003 bf16: 1024 threads a row 382 us, 256 237 us; 10^5 x 513 bf16: 64 threads 213 us, 8
+    // 72 us).
     const int per = 8 * (dtype == EDGEHIP_F32 ? TN_KEEP(EDGEHIP_F32) : TN_KEEP(EDGEHIP_BF16));
     int tpr = 1;
-    if (T.C > TN_ALONE) {
-        tpr = MODE == 1 ? 8 : 4;                                 // (writing only: wider runs of a row pay more)
+    if (T.C > tn_alone<MODE>(dtype)) {
+        // (only written: wider runs pay more where a row has more than 128 bytes; preference over 10^6 x 48 fp32: four threads
+        // 154 us, eight 135 us; over 10^6 x 33 bf16: 97 us, 107 us)
+        tpr = MODE == 1 && T.C > (dtype == EDGEHIP_F32 ? 32 : 64) ? 8 : 4;
         while (tpr < 64 && T.C > tpr * per) tpr *= 2;
         if (T.C > 64 * per) tpr = 256;
         while (tpr < 1024 && T.C > tpr * per) tpr *= 2;
     }
     const int rpb = (tpr < 256 ? 256 : tpr) / tpr;
     const dim3 grid((unsigned)((T.R + rpb - 1) / rpb)), block(tpr < 256 ? 256 : tpr);
-#define TN_TPR(DT, N) case N: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, N, MODE>), grid, block, 0, s, T)); break;
-#define TN_DT(DT) switch (T.C <= 8 ? 0 : tpr) { \
-        case 0: EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_rows<DT, 1, MODE, 1>), grid, block, 0, s, T)); break; \
-        TN_TPR(DT, 1) TN_TPR(DT, 4) TN_TPR(DT, 8) TN_TPR(DT, 16) TN_TPR(DT, 32) TN_TPR(DT, 64) TN_TPR(DT, 256) TN_TPR(DT, 512) TN_TPR(DT, 1024) }
-    if (dtype == EDGEHIP_F32) { TN_DT(EDGEHIP_F32) }
-    else if (dtype == EDGEHIP_BF16) { TN_DT(EDGEHIP_BF16) }
-    else { TN_DT(EDGEHIP_F16) }
-#undef TN_DT
-#undef TN_TPR
+    if (dtype == EDGEHIP_F32) tn_go<EDGEHIP_F32, MODE>(T, tpr, grid, block, s);
+    else if (dtype == EDGEHIP_BF16) tn_go<EDGEHIP_BF16, MODE>(T, tpr, grid, block, s);
+    else tn_go<EDGEHIP_F16, MODE>(T, tpr, grid, block, s);
     EH_LAUNCH_CHECK();
     return EDGEHIP_OK;
 }
@@ -564,7 +583,7 @@ extern "C" int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehi
     hipStream_t s = eh_stream(stream);
     T.logp = logp; T.rowstat = W.stat; T.dterm = W.dterm;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
-    if (T.C > TN_ALONE) TN_TRY(tn_sum<1>(T, s));             // (narrower rows: the row kernel makes the partials)
+    if (T.C > tn_alone<0>(Q->dtype)) TN_TRY(tn_sum<1>(T, s));             // (narrower rows: the row kernel makes the partials)
     F.loss = loss; F.kl = kl; F.clipped = clipped;
     EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
@@ -600,7 +619,7 @@ extern "C" int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgeh
     }
     T.logp = logp; T.dlogits = dlogits;
     TN_TRY(tn_launch<2>(Q->dtype, T, s));
-    if (T.C > TN_ALONE) TN_TRY(tn_sum<1>(T, s));
+    if (T.C > tn_alone<2>(Q->dtype)) TN_TRY(tn_sum<1>(T, s));
     F.scale = nullptr; F.loss = loss; F.kl = kl; F.clipped = clipped;
     EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_tn_policy_final<1>), dim3(F.S), dim3(256), 0, s, F));
     EH_LAUNCH_CHECK();
