@@ -439,25 +439,33 @@ __global__ __launch_bounds__(GN_THREADS(TPR), (TPR == GN_ROW ? 4 : GN_BWD_WAVES(
     if (A.gkind == EDGEHIP_GATE_VECTOR && A.want_gate) gn_flush<TPR>(ag, fl, p + 4 * plane, A.D, slot, t);
 }
 
-// partials -> sums, in block order.  blockIdx.y: which vector (a gate per group: which group); 64 columns x 16 strips
-struct gn_red { const float* part; int64_t plane; int nblk, D, rows_per_block; int64_t rows; void* out[5]; int dt[5]; const int32_t* row_ptr; };
+// partials -> sums, in block order.  blockIdx.x: which vector, then which group of the gate; 64 columns x 16 strips
+struct gn_red {
+    const float *part, *gpart;
+    int64_t plane;
+    int nblk, D, rows_per_block, vectors;
+    int64_t rows;
+    void *out[5], *dgate;
+    int dt[5], gdt;
+    const int32_t* row_ptr;
+};
 __global__ __launch_bounds__(1024) void k_gn_reduce(gn_red R) {
     __shared__ float s[16][64];
-    const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, col = blockIdx.x * 64 + c, v = blockIdx.y;
+    const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, col = blockIdx.y * 64 + c, v = blockIdx.x, g = v - R.vectors;
     int64_t b0 = 0, b1 = R.nblk;
     const float* src;
     void* out;
     int dt;
     int64_t at = col;
-    if (R.row_ptr) {
-        int64_t a = R.row_ptr[v], b = R.row_ptr[v + 1];
+    if (g >= 0) {
+        int64_t a = R.row_ptr[g], b = R.row_ptr[g + 1];
         if (a < 0) a = 0;
         if (b > R.rows) b = R.rows;
         b0 = a / R.rows_per_block;
         b1 = a < b ? (b - 1) / R.rows_per_block + 1 : b0;
-        src = R.part + (int64_t)v * R.D;                       // partial of (block, group): row block + group
-        out = R.out[0]; dt = R.dt[0];
-        at += (int64_t)v * R.D;
+        src = R.gpart + (int64_t)g * R.D;                      // partial of (block, group): row block + group
+        out = R.dgate; dt = R.gdt;
+        at += (int64_t)g * R.D;
     } else {
         out = R.out[v]; dt = R.dt[v];
         if (!out) return;
@@ -616,14 +624,11 @@ extern "C" int edgehip_gate_norm_bwd(const edgehip_gate_norm* G, const void* dh_
     R.part = A.part; R.plane = (int64_t)A.nblk * A.D; R.nblk = A.nblk; R.D = A.D; R.rows = G->rows; R.rows_per_block = A.rows_per_block;
     void* outs[5] = {dw_pre, db_pre, dw_post, db_post, G->gate_kind == EDGEHIP_GATE_VECTOR ? dgate : nullptr};
     for (int i = 0; i < 5; ++i) { R.out[i] = outs[i]; R.dt[i] = i < 4 ? G->param_dtype : G->gate_dtype; }
-    const int tiles = eh_cdiv(A.D, 64);
-    if (outs[0] || outs[1] || outs[2] || outs[3] || outs[4]) {
-        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_gn_reduce, dim3(tiles, 5), dim3(1024), 0, s, R));
-        EH_LAUNCH_CHECK();
-    }
-    if (G->gate_kind == EDGEHIP_GATE_GROUP && dgate) {
-        R.part = A.gpart; R.row_ptr = G->row_ptr; R.out[0] = dgate; R.dt[0] = G->gate_dtype;
-        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_gn_reduce, dim3(tiles, G->groups), dim3(1024), 0, s, R));
+    R.vectors = outs[0] || outs[1] || outs[2] || outs[3] || outs[4] ? 5 : 0;
+    R.gpart = A.gpart; R.row_ptr = G->row_ptr; R.dgate = dgate; R.gdt = G->gate_dtype;
+    const int sums = R.vectors + (G->gate_kind == EDGEHIP_GATE_GROUP && dgate ? G->groups : 0);
+    if (sums) {
+        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_gn_reduce, dim3(sums, eh_cdiv(A.D, 64)), dim3(1024), 0, s, R));
         EH_LAUNCH_CHECK();
     }
     return EDGEHIP_OK;

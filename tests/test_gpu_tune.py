@@ -343,3 +343,12 @@ def test_same_bits_on_other_streams_and_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, both())), k
+
+
+@pytest.mark.parametrize('rows,seqs,behind', [(16384, 512, 0), (16385, 512, 100), (16384, 514, 0), (20011, 4, 0), (3000, 700, 2000)])
+@pytest.mark.parametrize('classes,dtype', [(70, F32), (40, BF16), (5, F16)])
+def test_few_and_many_rows(rows, seqs, behind, classes, dtype):
+    """On both sides of where the sequences' sums are taken from the rows themselves."""
+    s = make(rows, classes, seqs, dtype, seed=rows + seqs, behind=behind)
+    check_policy(s)
+    check_pref(s, mean=True)
