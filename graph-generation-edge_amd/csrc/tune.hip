@@ -52,9 +52,11 @@ struct tn_rows {
 };
 
 __device__ static inline bool tn_counts(const tn_rows& T, int64_t r, int64_t& a) {
-    a = T.taken[r];
-    if (a < 0 || a >= T.C || (T.mask && !T.mask[r])) return false;
-    return !T.seq_ptr || (r >= T.seq_ptr[0] && r < T.seq_ptr[T.S]);
+    a = T.taken[r];                                              // (all requests at once, no branch between them)
+    bool on = (a >= 0) & (a < T.C);
+    if (T.mask) on &= T.mask[r] != 0;
+    if (T.seq_ptr) on &= (r >= T.seq_ptr[0]) & (r < T.seq_ptr[T.S]);
+    return on;
 }
 // the sequence of row r (r below seq_ptr[S])
 __device__ static inline int tn_seq(const int64_t* __restrict__ ptr, int S, int64_t r) {
@@ -102,9 +104,9 @@ __device__ static inline float tn_kl(float d) {
 }
 
 // the policy terms of one counted row; returns d term / d logp
-__device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, double logp, float& term, float& kl, bool& cut) {
+__device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, double logp, float old, float ref, float& term, float& kl, bool& cut) {
     const float A = T.adv[T.adv_per_row ? r : seq];
-    const double gain = logp - (double)T.old_logp[r];
+    const double gain = logp - (double)old;
     const float rho = expf((float)gain);
     cut = A > 0.0f ? gain > T.ln_hi : (A < 0.0f && gain < T.ln_lo);
     const float bound = A > 0.0f ? T.hi : T.lo;
@@ -112,7 +114,7 @@ __device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, d
     float d = cut ? 0.0f : -A * rho;
     kl = 0.0f;
     if (T.ref) {
-        const float gap = (float)((double)T.ref[r] - logp);
+        const float gap = (float)((double)ref - logp);
         kl = tn_kl(gap);
         term += T.kl_coef * kl;
         d -= T.kl_coef * (kl + gap);                             // exp(gap) - 1
@@ -131,13 +133,14 @@ __device__ static inline int tn_lane_seq(const tn_rows& T, int64_t r) {
     return r < T.R && r >= T.seq_ptr[0] && r < T.seq_ptr[T.S] ? tn_seq(T.seq_ptr, T.S, r) : -1;
 }
 
-// Sums over the lanes of a wave that share a sequence (g from tn_lane_seq; lanes that do not count have zeros): NV values,
-// and how many lanes have `cut` and `counts`.  The last lane of a run writes them as partial (wave w, sequence g), at slot
+// Sums over the lanes of a wave that share a sequence (g from tn_lane_seq; lanes that do not count have zeros): of v (WHAT 0:
+// nothing; 1: two values; 2: one), and how many lanes have `cut` and `counts`.  The last lane of a run writes them as partial (wave w, sequence g), at slot
 // w + g: along the rows one of the two grows by one at each border, so the slots are distinct and waves + sequences of
 // them are enough.
 #define TN_WAVE 64
-template <int NV>
-__device__ static inline void tn_wave_part(double (&v)[NV], bool cut, bool counts, int g, int64_t w, double* __restrict__ part) {
+template <int WHAT>
+__device__ static inline void tn_wave_part(double (&v)[WHAT == 1 ? 2 : 1], bool cut, bool counts, int g, int64_t w, double* __restrict__ part) {
+    constexpr int NV = WHAT == 0 ? 0 : WHAT == 1 ? 2 : 1;
     const int lane = threadIdx.x & 63;
     const int before = __shfl_up(g, 1, 64), after = __shfl_down(g, 1, 64);
     const uint64_t starts = __ballot(lane == 0 || before != g);
@@ -164,7 +167,7 @@ __device__ static inline void tn_wave_part(double (&v)[NV], bool cut, bool count
     if (g >= 0 && (lane == 63 || after != g)) {
         double* p = part + (w + g) * 4;
         p[0] = NV > 0 ? v[0] : 0.0;
-        p[1] = NV > 1 ? v[NV - 1] : 0.0;
+        p[1] = NV > 1 ? v[WHAT == 1] : 0.0;
         p[2] = (double)__popcll(cuts & run);
         p[3] = (double)__popcll(all & run);
     }
@@ -247,6 +250,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     const int C = T.C;
     const int64_t base = r * T.ld;
     int64_t a = -1;
+    float old = 0.0f, ref = 0.0f;
+    if (MODE != 1 && T.old_logp && r < T.R) {
+        old = T.old_logp[r];
+        if (T.ref) ref = T.ref[r];
+    }
     const bool counts = r < T.R && tn_counts(T, r, a);
     constexpr int KEEP = MODE == 1 ? 1 : TPR == 1 ? PIECES : MODE == 2 ? TN_KEEP(DT) : 1;
     eh_raw8<DT> keep[KEEP];
@@ -264,6 +272,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         }
         tn_add8<(TPR <= 64)>(m, s, v);
     };
+    float only[8];                                                // 8 classes or less: the row
+    if (!WHOLE && r < T.R) eh_load8<DT>(row, 0, C, only, -__builtin_inff());
     const bool kept = MODE != 1 && WHOLE && C <= TPR * 8 * KEEP;
     if (MODE != 1) {
         if (counts) {
@@ -281,12 +291,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
                     keep[k].get(v);
                     if (c < C) add(v, c);
                 }
-            } else {
+            } else if (WHOLE) {
                 for (int c = t * 8; c < C; c += TPR * 8) {
                     float v[8];
-                    eh_load8<DT>(row, start(c), WHOLE ? 8 : C, v, -__builtin_inff());
+                    eh_load8<DT>(row, start(c), 8, v);
                     add(v, c);
                 }
+            } else {
+                tn_add8<true>(m, s, only);
             }
             tn_row_merge<TPR>(m, s, lds);                         // (a row counts for all of its threads or none)
         }
@@ -301,7 +313,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
             inv = 1.0f / s;
             if (T.old_logp) {
                 if (TPR > 1) seq = tn_wave_seq<RPW>(T.seq_ptr, T.S, r);
-                d = tn_policy(T, r, seq, logp, term, kl, cut);
+                d = tn_policy(T, r, seq, logp, old, ref, term, kl, cut);
                 if (MODE == 2) coef = (float)((double)d * tn_scale(T, seq));
             }
         }
@@ -318,7 +330,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         }
         if (TPR == 1 && T.old_logp) {
             double v[2] = {(double)term, (double)kl};
-            tn_wave_part<2>(v, cut, counts, seq, r / TN_WAVE, T.part);
+            tn_wave_part<1>(v, cut, counts, seq, r / TN_WAVE, T.part);
         }
         if (TPR == 1 && r >= T.R) return;
     } else if (counts) {
@@ -340,7 +352,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
                     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
                 } else {
                     if (kept) keep[k].get(v);
-                    else eh_load8<DT>(row, c, WHOLE ? 8 : C, v);
+                    else if (WHOLE) eh_load8<DT>(row, c, 8, v);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = only[i];
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = f * __builtin_amdgcn_exp2f((v[i] - m) * TN_LOG2E);
                     if (a >= c && a < c + 8) {
@@ -361,16 +377,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
 template <int WHAT>
 __global__ __launch_bounds__(256) void k_tn_part(tn_rows T) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int g = tn_lane_seq(T, r);
-    int64_t cls;
-    const bool counts = g >= 0 && tn_counts(T, r, cls);
     double v[WHAT == 1 ? 2 : 1] = {0.0};
-    bool cut = false;
-    if (counts) {
+    bool cut = false, counts = false;
+    if (r < T.R) {                                                // requested before the search
+        int64_t cls;
+        counts = tn_counts(T, r, cls);
         if (WHAT == 1) { v[0] = T.term[r]; v[WHAT == 1] = T.kl[r]; cut = T.clipped[r]; }
         if (WHAT == 2) v[0] = T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
     }
-    tn_wave_part(v, cut, counts, g, r / TN_WAVE, T.part);
+    const int g = tn_lane_seq(T, r);
+    if (!counts) {
+        v[0] = v[WHAT == 1] = 0.0;
+        cut = false;
+    }
+    tn_wave_part<WHAT>(v, cut, counts, g, r / TN_WAVE, T.part);
 }
 
 struct tn_final {
@@ -424,10 +444,12 @@ __device__ static inline void tn_total(const tn_final& F, const tn_rows& T, int 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
-        if (DIRECT) {
-            for (int w = 4; w < 16; w += 4) v[i] += (red[w][i] + red[w + 1][i]) + (red[w + 2][i] + red[w + 3][i]);
+    for (int i = 0; i < 4; ++i) v[i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    if (DIRECT) {
+#pragma unroll 1
+        for (int w = 4; w < 16; w += 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += (red[w][i] + red[w + 1][i]) + (red[w + 2][i] + red[w + 3][i]);
         }
     }
 }
