@@ -416,14 +416,14 @@ __device__ static inline void tn_total(const tn_final& F, const tn_rows& T, int 
     if (DIRECT) {
 #pragma unroll 4
         for (int64_t r = a + threadIdx.x; r < b; r += 1024) {
+            double x = 0.0, y = 0.0;
+            bool cut = false;
+            if (WHAT == 1) { x = T.term[r]; y = T.kl[r]; cut = T.clipped[r]; }
+            if (WHAT == 2) x = T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0);
             int64_t cls;
             const bool counts = tn_counts(T, r, cls);
-            if (WHAT == 1) {
-                v[0] += counts ? (double)T.term[r] : 0.0;
-                v[1] += counts ? (double)T.kl[r] : 0.0;
-                v[2] += counts && T.clipped[r] ? 1.0 : 0.0;
-            }
-            if (WHAT == 2) v[0] += counts ? T.logp64[r] - (T.ref ? (double)T.ref[r] : 0.0) : 0.0;
+            if (WHAT) v[0] += counts ? x : 0.0;
+            if (WHAT == 1) { v[1] += counts ? y : 0.0; v[2] += counts && cut ? 1.0 : 0.0; }
             v[3] += counts ? 1.0 : 0.0;
         }
     } else if (a < b) {
