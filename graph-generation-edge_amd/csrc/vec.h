@@ -2,7 +2,7 @@
 //
 // gfx950 takes 16-byte global accesses at any element-aligned address, so a row of odd length or a view that starts in
 // the middle of a line is read with the same vector accesses as an aligned one: the vector types below only promise the
-// alignment of their element.  The last, partial vector of a row goes element by element.
+// alignment of their element.  What a row's last vector does with the values it lacks: eh_place, or eh_load8 value by value.
 #pragma once
 #include "common.h"
 
