@@ -290,3 +290,45 @@ def test_second_derivatives_are_refused():
         first, = torch.autograd.grad(out.square().sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match='once_differentiable'):
             first.sum().backward()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values in a tensor: the last rows come out as they do in a tensor of their own, bit for bit."""
+    import edgehip
+    rows, dim, last = (1 << 20) + 5003, 2048, 300
+    g = torch.Generator(device='cuda').manual_seed(11)
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device='cuda')
+    for a in range(0, rows, 1 << 17):
+        x[a:a + (1 << 17)] = torch.randn(min(1 << 17, rows - a), dim, generator=g, device='cuda')
+    tail = x[-last:].clone()
+    w = torch.rand(dim, generator=g, device='cuda') + 0.5
+    ho, y, st = edgehip.block.gate_norm_fwd(x, x, w_pre=w, gate=w, want_stats=True)
+    ho1, y1, st1 = edgehip.block.gate_norm_fwd(tail, tail, w_pre=w, gate=w, want_stats=True)
+    assert torch.equal(ho[-last:], ho1) and torch.equal(y[-last:], y1) and torch.equal(st[-last:], st1)
+    del ho
+    b = edgehip.block.gate_norm_bwd(y, x, x, x, st, w_pre=w, gate=w)
+    b1 = edgehip.block.gate_norm_bwd(y1, tail, tail, tail, st1, w_pre=w, gate=w)
+    assert torch.equal(b['dh'][-last:], b1['dh']) and torch.equal(b['dz'][-last:], b1['dz'])
+    del b, y
+    a, p = edgehip.ckpt8.act8_fwd(x)
+    a1, p1 = edgehip.ckpt8.act8_fwd(tail)
+    assert torch.equal(a[-last:], a1) and torch.equal(p.codes[-last:], p1.codes) and torch.equal(p.exps[-last:], p1.exps)
+    assert torch.equal(edgehip.ckpt8.act8_bwd(x, p)[-last:], edgehip.ckpt8.act8_bwd(tail, p1))
+    # the weight's gradient: dY is zero but for the last rows, so only they can show
+    a.zero_()
+    a[-last:] = tail
+    dw, db = edgehip.ckpt8.linear8_bwd_weight(a, p)
+    dw1, db1 = edgehip.ckpt8.linear8_bwd_weight(tail, p1)
+    # fp32 sums of 300 exact products in another order: 300 half steps of their sizes' sum
+    size = tail.float().abs().t() @ p1.unpack(torch.float32).abs()
+    assert bool(((dw - dw1).abs() <= 600 * 2.0 ** -24 * size).all()) and bool(((db - db1).abs() <= 600 * 2.0 ** -24 * tail.float().abs().sum(0)).all())
+    del a, p, dw
+    taken = torch.randint(0, dim, (rows,), generator=g, device='cuda')
+    lp = edgehip.row_logp(x, taken)
+    assert torch.equal(lp[-last:], edgehip.row_logp(tail, taken[-last:]))
+    ptr = torch.tensor([0, rows - last, rows], device='cuda')
+    adv = torch.tensor([0.0, 1.5], device='cuda')
+    r = edgehip.policy_loss_grad(x, taken, lp, adv, ptr, reduce='sum')
+    r1 = edgehip.policy_loss_grad(tail, taken[-last:].contiguous(), lp[-last:].contiguous(), adv[1:], torch.tensor([0, last], device='cuda'),
+                                  reduce='sum', weight=torch.tensor([0.5], device='cuda'))
+    assert torch.equal(r.dlogits[-last:], r1.dlogits) and not bool(r.dlogits[:last].any())
