@@ -310,7 +310,7 @@ template <int DT, int CW> struct dw_y {
 template <int DT, int T>
 __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __restrict__ dY, const int8_t* __restrict__ codes,
                                                                 const int8_t* __restrict__ exps, int64_t M, int N, int K, int KG,
-                                                                int64_t rows_per_split, int nt, int kt, float* __restrict__ out,
+                                                                int64_t rows_per_split, int nt, int kt, int kb, float* __restrict__ out,
                                                                 float* __restrict__ db) {
     constexpr int P = dw_planes<DT>::value, BM = dw_rows<DT>::value, CW = T * BM >= 8192 ? 4 : 2, W = T / 2, F = W / 32;
     constexpr int MB = 256 / (T / CW), U = BM / 8 / MB;         // m-blocks staged at once, times the U pieces of a thread
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
     int turn = 0, chunk = 0;
     // the column sums of the chunk at row m, which register set `set` holds
     auto count_db = [&](int64_t m, int set) {
-        if (db && chunk % kt == ktile) {
+        if (db && chunk % kb == ktile) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
                 const int n = n0 + wn + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh, k = k0 + wk + j * 32 + fr;
                 if (n < N && k < K) o[(int64_t)n * K + k] = acc[i][j][r];
             }
-    if (db) {
+    if (db && ktile < kb) {
         // the MB threads that hold one column's sums, through LDS
         __syncthreads();
         float* red = reinterpret_cast<float*>(img[0]);
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void k_ck_dw(const void* __r
             float s = 0.0f;
 #pragma unroll
             for (int b = 0; b < MB; ++b) s += red[b * T + tid];
-            db[((int64_t)blockIdx.y * kt + ktile) * N + n0 + tid] = s;
+            db[((int64_t)blockIdx.y * kb + ktile) * N + n0 + tid] = s;
         }
     }
 }
@@ -549,20 +549,16 @@ __global__ __launch_bounds__(256) void k_ck_dw_thin(const void* __restrict__ dY,
     if (db && k == 0) db[(int64_t)blockIdx.y * N + n] = b;
 }
 
-// Sums of the partial results, in order: 64 columns of four x 16 strips of partials a block; the strips meet in LDS.  The
-// first `blocks` blocks add the tiles, the rest db.
-__global__ __launch_bounds__(1024) void k_ck_dw_sum(const float* __restrict__ part, int64_t n, int parts, float* __restrict__ out,
-                                                    const float* __restrict__ part_b, int64_t nb, int parts_b, float* __restrict__ out_b,
-                                                    int blocks) {
-    __shared__ float s[16][256 + 16];
-    const bool second = (int)blockIdx.x >= blocks;
-    const float* src = second ? part_b : part;
-    const int64_t len = second ? nb : n, at = ((int64_t)blockIdx.x - (second ? blocks : 0)) * 256 + (threadIdx.x & 63) * 4;
-    const int np = second ? parts_b : parts, strip = threadIdx.x >> 6;
+// Sums of partial results, in order: LANES columns of four x STRIPS strips of partials a block; the strips meet in LDS.
+template <int STRIPS, int LANES>
+__device__ static inline void dw_sum(const float* __restrict__ src, int64_t len, int np, float* __restrict__ out, int64_t block, float* lds) {
+    constexpr int PAD = LANES * 4 + 16;
+    const int lane = threadIdx.x % LANES, strip = threadIdx.x / LANES;
+    const int64_t first = block * LANES * 4, at = first + lane * 4;
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const int left = at < len ? (len - at < 4 ? (int)(len - at) : 4) : 0;
 #pragma unroll 4
-    for (int z = strip; z < np; z += 16) {
+    for (int z = strip; z < np; z += STRIPS) {
         const float* p = src + z * len + at;
         if (left == 4) {
             const eh_f32x4u v = *reinterpret_cast<const eh_f32x4u*>(p);
@@ -572,20 +568,36 @@ __global__ __launch_bounds__(1024) void k_ck_dw_sum(const float* __restrict__ pa
             for (int i = 0; i < left; ++i) a[i] += p[i];
         }
     }
+    if (STRIPS == 1) {
+        if (left == 4) *reinterpret_cast<eh_f32x4u*>(out + at) = eh_f32x4u{a[0], a[1], a[2], a[3]};
+        else for (int i = 0; i < left; ++i) out[at + i] = a[i];
+        return;
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[strip][(threadIdx.x & 63) * 4 + i] = a[i];
+    for (int i = 0; i < 4; ++i) lds[strip * PAD + lane * 4 + i] = a[i];
     __syncthreads();
     const int c = threadIdx.x;
-    const int64_t col = ((int64_t)blockIdx.x - (second ? blocks : 0)) * 256 + c;
-    if (c < 256 && col < len) {
+    if (c < LANES * 4 && first + c < len) {
         float v = 0.0f;
 #pragma unroll
-        for (int z = 0; z < 16; ++z) v += s[z][c];
-        (second ? out_b : out)[col] = v;
+        for (int z = 0; z < STRIPS; ++z) v += lds[z * PAD + c];
+        out[first + c] = v;
     }
 }
+// The first `blocks` blocks add the tiles, the rest db.  One strip for few partials, or where the values fill the chip
+// anyway (256 rows of 1024 x 1024 bf16, the whole gradient: 16 strips 31 us, one 24 us).
+static bool dw_one_strip(int parts, int64_t n) { return parts <= 4 || (parts <= 16 && n >= (1 << 18)); }
+template <int STRIPS, int LANES>
+__global__ __launch_bounds__(STRIPS * LANES) void k_ck_dw_sum(const float* __restrict__ part, int64_t n, int parts, float* __restrict__ out,
+                                                              const float* __restrict__ part_b, int64_t nb, int parts_b,
+                                                              float* __restrict__ out_b, int blocks) {
+    constexpr int LB = STRIPS * LANES / 16;
+    __shared__ float lds[16 * (LB * 4 + 16)];
+    if ((int)blockIdx.x < blocks) dw_sum<STRIPS, LANES>(part, n, parts, out, blockIdx.x, lds);
+    else dw_sum<16, LB>(part_b, nb, parts_b, out_b, (int64_t)blockIdx.x - blocks, lds);
+}
 
-struct dw_plan { int tile, nt, kt, splits; int64_t rows; };
+struct dw_plan { int tile, nt, kt, splits, kb; int64_t rows; };
 // The tile and the splits of the rows: the chip holds one block of the larger tile a CU, two of the smaller
 static dw_plan dw_choose(int64_t M, int N, int K) {
     dw_plan p;
@@ -602,6 +614,11 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
     int64_t s = tiles >= room ? 1 : room / tiles;
     if (s > most) s = most;
     if (s < 1) s = 1;
+    // Up to 128 rows one block goes over all of them and the first k-tile makes all of db: no partials, no second launch
+    // (128 rows of 1024 x 1024 / 4096 x 500 bf16: split 19 / 24 us, whole 16 / 17 us; 16 rows of 100 x 100 15 us, 12 us;
+    // fp32 512 x 512: 19 us, 22 us).
+    p.kb = p.kt;
+    if (M <= 128) s = p.kb = 1;
     p.rows = ((M + s - 1) / s + 63) / 64 * 64;
     if (p.rows < 64) p.rows = 64;
     p.splits = (int)((M + p.rows - 1) / p.rows);
@@ -617,7 +634,7 @@ static int dw_check(int32_t dtype, int64_t M, int32_t N, int32_t K) {
 
 static size_t dw_floats(const dw_plan& p, int N, int K, size_t& db_at) {
     db_at = p.splits > 1 ? (size_t)p.splits * N * K : 0;
-    return db_at + (p.splits * p.kt > 1 ? (size_t)p.splits * p.kt * N : 0);
+    return db_at + (p.splits * p.kb > 1 ? (size_t)p.splits * p.kb * N : 0);
 }
 
 extern "C" size_t edgehip_linear8_workspace_bytes(int32_t dtype, int64_t M, int32_t N, int32_t K) {
@@ -638,12 +655,12 @@ extern "C" int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const i
     EH_CHECK_ARG(need == 0 || (ws && ((uintptr_t)ws & 3) == 0));
     hipStream_t s = eh_stream(stream);
     float* base = reinterpret_cast<float*>(ws);
-    const bool many_b = p.splits * p.kt > 1;
+    const bool many_b = p.splits * p.kb > 1;
     float* part = p.splits > 1 ? base : dW;
     float* pdb = !db ? nullptr : many_b ? base + at : db;
     const dim3 grid(p.nt * p.kt, p.splits), block(256);
     const int KG = (K + CK_GROUP - 1) / CK_GROUP;
-#define DW_GO(DT, T) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw<DT, T>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, p.nt, p.kt, part, pdb))
+#define DW_GO(DT, T) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw<DT, T>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, p.nt, p.kt, p.kb, part, pdb))
 #define DW_THIN(DT) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw_thin<DT>), grid, block, 0, s, dY, codes, exps, M, N, K, KG, p.rows, part, pdb))
 #define DW_TILE(DT) do { if (p.tile == 256) DW_GO(DT, 256); else if (p.tile) DW_GO(DT, 128); else DW_THIN(DT); } while (0)
     if (dtype == EDGEHIP_F32) DW_TILE(EDGEHIP_F32);
@@ -654,11 +671,15 @@ extern "C" int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const i
 #undef DW_GO
     EH_LAUNCH_CHECK();
     const int64_t n = (int64_t)N * K;
-    const int blocks = p.splits > 1 ? eh_cdiv(n, 256) : 0, more = db && many_b ? eh_cdiv(N, 256) : 0;
+    const bool few = dw_one_strip(p.splits, n);
+    const int blocks = p.splits > 1 ? eh_cdiv(n, few ? 1024 : 256) : 0, more = db && many_b ? eh_cdiv(N, few ? 64 : 256) : 0;
+#define DW_SUM(S, L) EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL((k_ck_dw_sum<S, L>), dim3(blocks + more), dim3(S * L), 0, s, part, n, p.splits, dW, pdb, \
+                                                               (int64_t)N, p.splits * p.kb, db, blocks))
     if (blocks + more) {
-        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_ck_dw_sum, dim3(blocks + more), dim3(1024), 0, s, part, n, p.splits, dW, pdb, (int64_t)N,
-                                                  p.splits * p.kt, db, blocks));
+        if (few) DW_SUM(1, 256);
+        else DW_SUM(16, 64);
         EH_LAUNCH_CHECK();
     }
+#undef DW_SUM
     return EDGEHIP_OK;
 }
