@@ -233,7 +233,7 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 // different slots, and a fragment (32 consecutive columns) still reads 32 consecutive pieces: no bank conflicts.
 //
 // A block owns a T x T tile of dW and a run of rows; four waves, T/2 x T/2 each.  T = 256 needs half the LDS reads per flop
-// of T = 128 and is taken where both sides are wider than 128; its 256 accumulators leave one wave a SIMD, so everything
+// of T = 128 and is taken for large products (dw_choose); its 256 accumulators leave one wave a SIMD, so everything
 // else is placed between its matrix instructions: two LDS images, and while a chunk of BM rows is multiplied, the next
 // one's registers (requested a chunk earlier) are turned and written and the one after is requested, in one run of
 // instructions without a branch; one barrier a chunk, which waits for LDS only, so that the requests stay in flight
@@ -585,7 +585,7 @@ __device__ static inline void dw_sum(const float* __restrict__ src, int64_t len,
     }
 }
 // The first `blocks` blocks add the tiles, the rest db.  One strip for few partials, or where the values fill the chip
-// anyway (256 rows of 1024 x 1024 bf16, the whole gradient: 16 strips 31 us, one 24 us).
+// anyway (1024 rows of 1024 x 1024 bf16, the whole gradient: 16 strips 40 us, one 30 us).
 static bool dw_one_strip(int parts, int64_t n) { return parts <= 4 || (parts <= 16 && n >= (1 << 18)); }
 template <int STRIPS, int LANES>
 __global__ __launch_bounds__(STRIPS * LANES) void k_ck_dw_sum(const float* __restrict__ part, int64_t n, int parts, float* __restrict__ out,
@@ -598,10 +598,15 @@ __global__ __launch_bounds__(STRIPS * LANES) void k_ck_dw_sum(const float* __res
 }
 
 struct dw_plan { int tile, nt, kt, splits, kb; int64_t rows; };
-// The tile and the splits of the rows: the chip holds one block of the larger tile a CU, two of the smaller
+// The tile and the splits of the rows: the chip holds one block of the larger tile a CU, two of the smaller.  The larger one
+// pays where its tiles fill the chip, or each of a few has thousands of rows (tiles x 64-row pieces: 4096); below, four times
+// the blocks do (4096 rows of 1024 x 1024 bf16: larger 39 us, smaller 29 us; 1024 of 2048 x 2048: 40, 33 us; 2048 of 2048 x
+// 2048 fp32: 73, 74 us; 512 of 4096 x 4096 bf16: 36, 40 us).
 static dw_plan dw_choose(int64_t M, int N, int K) {
     dw_plan p;
-    p.tile = N > 128 && K > 128 ? 256 : 128;
+    const int64_t most = (M + 63) / 64;
+    const int64_t large = (int64_t)eh_cdiv(N, 256) * eh_cdiv(K, 256);
+    p.tile = N > 128 && K > 128 && large * most >= (large >= 256 ? 1024 : 4096) ? 256 : 128;
     p.nt = eh_cdiv(N, p.tile);
     p.kt = eh_cdiv(K, p.tile);
     if (N < 4 || K < 4) {                        // k_ck_dw_thin: blocks of 256 values
@@ -609,14 +614,13 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
         p.nt = eh_cdiv((int64_t)N * K, 256);
         p.kt = 1;
     }
-    const int64_t tiles = (int64_t)p.nt * p.kt, most = (M + 63) / 64;
+    const int64_t tiles = (int64_t)p.nt * p.kt;
     const int64_t room = p.tile == 256 ? 256 : 512;      // blocks the chip holds at once
     int64_t s = tiles >= room ? 1 : room / tiles;
     if (s > most) s = most;
     if (s < 1) s = 1;
     // Up to 128 rows one block goes over all of them and the first k-tile makes all of db: no partials, no second launch
-    // (128 rows of 1024 x 1024 / 4096 x 500 bf16: split 19 / 24 us, whole 16 / 17 us; 16 rows of 100 x 100 15 us, 12 us;
-    // fp32 512 x 512: 19 us, 22 us).
+    // (16 rows of 64 x 1000: 15 us, 12 us a call; 128 rows of 100 x 100 fp32: 9.3 us, 10.4 us on the device, 15 us, 12 us a call).
     p.kb = p.kt;
     if (M <= 128) s = p.kb = 1;
     p.rows = ((M + s - 1) / s + 63) / 64 * 64;

@@ -323,3 +323,20 @@ def test_a_layer_keeps_its_type_inside_autocast():
         grads = torch.autograd.grad(z, [x, w], torch.ones_like(z))
     assert z.dtype == F32 and torch.equal(y, z)
     assert all(torch.equal(a, c) for a, c in zip(grads, torch.autograd.grad(y, [x, w], torch.ones_like(y))))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,n,k', [(1030, 4099, 4100), (70001, 300, 500), (66000, 1000, 257), (131101, 129, 258), (70000, 512, 256), (9001, 300, 500),
+                                   (129, 700, 1100), (300, 2048, 513)])
+def test_weight_gradient_large(dtype, m, n, k):
+    """Products large enough for the larger tile, and some just below; tolerances as above."""
+    import edgehip
+    x, dy = sample(m, k, dtype, seed=m), torch.randn(m, n, device='cuda').to(dtype)
+    p = edgehip.pack8(x)
+    dw, db = edgehip.ckpt8.linear8_bwd_weight(dy, p)
+    q, d = p.unpack(F32).double(), dy.double()
+    want, size = d.t().contiguous() @ q, d.abs().t().contiguous() @ q.abs()
+    assert bool(((dw.double() - want).abs() <= (m / 16 + 80) * U * size + 1e-30).all())
+    assert bool(((db.double() - d.sum(0)).abs() <= (m / 8 + 80) * U * d.abs().sum(0)).all())
+    again, db2 = edgehip.ckpt8.linear8_bwd_weight(dy, p)
+    assert torch.equal(again, dw) and torch.equal(db, db2)
