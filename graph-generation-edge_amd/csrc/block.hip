@@ -12,7 +12,7 @@
 // Bound by HBM: 14 flops a value forward, 26 backward.  Everything between the reads of h, z (dh', dy) and the writes
 // of h', y (dh, dz) stays in registers: a thread owns 8 columns of a row (one 16-byte access of a 16-bit type), the
 // threads of a row meet in a wave reduction (and, where it has more than 64, in LDS).  16384 x 4096 bf16: forward 104 us,
-// 5.2 TB/s, backward 177 us, 4.5 TB/s (+ 8 us for the partials), against 5.1 TB/s of a large copy; 78208 x 64 fp32 with a
+// 5.2 TB/s, backward 177 us, 4.5 TB/s (+ 7 us for the partials), against 5.1 TB/s of a large copy; 78208 x 64 fp32 with a
 // gate per graph: 21 us and 32 us (3.8 TB/s), there the start and end of the launches tell.  The backward pass recomputes u, h' from
 // h and z instead of reading a kept h': the same bytes, and the gradient is that of the unrounded h'.  y, too, is made
 // from the unrounded h'.  All statistics and sums are fp32; each output is rounded once.
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(GN_THREADS(TPR), (TPR == GN_ROW ? 4 : GN_BWD_WAVES(
     if (A.gkind == EDGEHIP_GATE_VECTOR && A.want_gate) gn_flush<TPR>(ag, fl, p + 4 * plane, A.D, slot, t);
 }
 
-// partials -> sums, in block order.  blockIdx.x: which vector, then which group of the gate; 64 columns x 16 strips
+// partials -> sums, in block order.  blockIdx.x: which vector, then which group of the gate; 32 columns x 32 strips
 struct gn_red {
     const float *part, *gpart;
     int64_t plane;
@@ -450,8 +450,8 @@ struct gn_red {
     const int32_t* row_ptr;
 };
 __global__ __launch_bounds__(1024) void k_gn_reduce(gn_red R) {
-    __shared__ float s[16][64];
-    const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, col = blockIdx.y * 64 + c, v = blockIdx.x, g = v - R.vectors;
+    __shared__ float s[32][33];
+    const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, col = blockIdx.y * 32 + c, v = blockIdx.x, g = v - R.vectors;
     int64_t b0 = 0, b1 = R.nblk;
     const float* src;
     void* out;
@@ -473,14 +473,14 @@ __global__ __launch_bounds__(1024) void k_gn_reduce(gn_red R) {
     }
     float a = 0.0f;
     if (col < R.D) {
-#pragma unroll 4
-        for (int64_t b = b0 + strip; b < b1; b += 16) a += src[b * R.D + col];
+#pragma unroll 8
+        for (int64_t b = b0 + strip; b < b1; b += 32) a += src[b * R.D + col];
     }
     s[strip][c] = a;
     __syncthreads();
     if (strip == 0 && col < R.D) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) a += s[i][c];
+        for (int i = 1; i < 32; ++i) a += s[i][c];
         eh_store1_any(out, dt, at, a);
     }
 }
@@ -628,7 +628,7 @@ extern "C" int edgehip_gate_norm_bwd(const edgehip_gate_norm* G, const void* dh_
     R.gpart = A.gpart; R.row_ptr = G->row_ptr; R.dgate = dgate; R.gdt = G->gate_dtype;
     const int sums = R.vectors + (G->gate_kind == EDGEHIP_GATE_GROUP && dgate ? G->groups : 0);
     if (sums) {
-        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_gn_reduce, dim3(sums, eh_cdiv(A.D, 64)), dim3(1024), 0, s, R));
+        EH_PROF(EH_K_TRAIN, s, hipLaunchKernelGGL(k_gn_reduce, dim3(sums, eh_cdiv(A.D, 32)), dim3(1024), 0, s, R));
         EH_LAUNCH_CHECK();
     }
     return EDGEHIP_OK;
