@@ -245,7 +245,7 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 //
 // The rows are split where the tiles alone do not fill the chip; partial tiles go to the workspace and are added in
 // order by k_ck_dw_sum.  db: the block of k-tile j adds up the chunks with number j modulo the k-tiles, so that this work
-// is spread over them; partials by (split, k-tile).
+// is spread over them (up to 128 rows: the first block's alone); partials by (split, k-tile).
 // ------------------------------------------------------------------------------------------------------------------
 #define CK_BARRIER() asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory")
 
