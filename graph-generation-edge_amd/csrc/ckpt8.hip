@@ -557,16 +557,23 @@ __device__ static inline void dw_sum(const float* __restrict__ src, int64_t len,
     const int64_t first = block * LANES * 4, at = first + lane * 4;
     float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const int left = at < len ? (len - at < 4 ? (int)(len - at) : 4) : 0;
-#pragma unroll 4
-    for (int z = strip; z < np; z += STRIPS) {
-        const float* p = src + z * len + at;
-        if (left == 4) {
-            const eh_f32x4u v = *reinterpret_cast<const eh_f32x4u*>(p);
+    if (len >= 4) {                                              // the last four columns are read whole and moved down
+        const int64_t from = at + 4 <= len ? at : len - 4;
+#pragma unroll 8
+        for (int z = strip; z < np; z += STRIPS) {
+            const eh_f32x4u v = *reinterpret_cast<const eh_f32x4u*>(src + z * len + from);
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] += v[i];
-        } else {
-            for (int i = 0; i < left; ++i) a[i] += p[i];
         }
+        const int by = left ? (int)(at - from) : 0;
+        const float a1 = a[1], a2 = a[2], a3 = a[3];
+        a[0] = by == 1 ? a1 : by == 2 ? a2 : by == 3 ? a3 : a[0];
+        a[1] = by == 1 ? a2 : by == 2 ? a3 : a1;
+        a[2] = by == 1 ? a3 : a2;
+    } else if (left) {
+        for (int z = strip; z < np; z += STRIPS)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) a[i] += src[z * len + (i < left ? i : 0)];
     }
     if (STRIPS == 1) {
         if (left == 4) *reinterpret_cast<eh_f32x4u*>(out + at) = eh_f32x4u{a[0], a[1], a[2], a[3]};
