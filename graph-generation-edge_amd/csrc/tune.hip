@@ -13,9 +13,10 @@
 // Bound by HBM for many classes: 2 bytes a bf16 logit in, 2 out.  The one-pass form reads a row once, keeps it in
 // registers while its sum is taken, and writes its gradient; rows too long for that are read a second time right after
 // the first, from cache.  The log-probability and its differences (to old, to ref) are fp64, a few operations a row:
-// their error would enter every value of the gradient.  What follows from a difference is fp32 in forms that do not cancel,
-// the exponentials of a row are fp32 (1e-7 relative each), their sum is better than each.  Whether the clip binds is
-// decided on the logarithm in fp64.  Sums over a sequence's rows are fp64, in a fixed order.
+// their error would enter every value of the gradient.  What follows from a difference is fp32 in forms that do not cancel.
+// A row's exponentials are summed in fp64 (rows of more than 64 threads: eights of them), so that the sum is better than each:
+// a log-probability is off by 1e-8.  Whether the clip binds is decided on the logarithm in fp64.  Sums over a sequence's
+// rows are fp64, in a fixed order.
 #include "common.h"
 #include "prof.h"
 #include "vec.h"
@@ -173,67 +174,101 @@ __device__ static inline void tn_wave_part(double (&v)[WHAT == 1 ? 2 : 1], bool 
     }
 }
 
-// exp(x), x <= 0 or NaN.  The fp32 constant log2(e) alone is 1.3e-8 off: every term of a row would be off to the same side by
-// that times |x|, and a preference's margin is the difference of hundreds of such rows.  With the constant's second part the
-// error of a term is that of rounding x log2(e), to either side; many terms average it.  FEW: rows of few classes have no
-// many, there the whole part is split off first and a term is right to 2 ulp (twice the work).
-template <bool FEW>
+// e^x, x <= 0 or NaN, in fp64 to 3.5e-8 (rms 6e-9, mean below 2e-10).  e^x = 2^n (1 + q): n = rint(x log2 e), r = x - n ln 2, ln 2
+// as 16 bits (n times them is exact) and the rest; q = e^r - 1 = r + r^2 P(r) in fp32, where its rounding is at most 2^-26; P
+// has the smallest largest error over |r| <= ln 2 / 2, 5e-10.  A row of few classes has no many terms to average over and a
+// preference's margin is the difference of sums over many such rows: rounded to fp32 and added up there, a row's
+// log-probability was off by 3e-8 to 7e-8, all margins by that times the root of their rows and more.
+__device__ static inline double tn_exp64(float x) {
+    x = x < -150.0f ? -150.0f : x;                               // (-inf; NaN stays)
+    const float t = __builtin_fmaf(x, 1.44269504f, 12582912.0f), n = t - 12582912.0f;     // n in t's last bits
+    const float r1 = __builtin_fmaf(n, -0.693145751953125f, x), c = n * -1.42860682e-6f, r = r1 + c;
+    float p = 0.00020303126f;
+    p = __builtin_fmaf(p, r, 0.001393498f);
+    p = __builtin_fmaf(p, r, 0.008332706f);
+    p = __builtin_fmaf(p, r, 0.04166643f);
+    p = __builtin_fmaf(p, r, 0.16666669f);
+    p = __builtin_fmaf(p, r, 0.5f);
+    // (c not by way of r: x - n 16 bits lies on r's grid, so that c would be rounded to the same side for all x of an n)
+    const float q = r1 + __builtin_fmaf(r * r, p, c);
+    return __builtin_ldexp(1.0 + (double)q, __float_as_int(t) - 0x4b400000);
+}
+// The same in fp32 by the hardware's power of two, for rows of many classes.  The fp32 constant log2(e) alone is 1.3e-8 off:
+// every term of a row would be off to the same side by that times |x|.  With the constant's second part the error of a term
+// is that of rounding x log2(e), to either side, and the instruction's own (mean -3e-9).
 __device__ static inline float tn_exp(float x) {
     constexpr float HI = 1.44269502162933349609f, LO = 1.92596298909109e-8f;
-    if (!FEW) return __builtin_amdgcn_exp2f(__builtin_fmaf(x, HI, x * LO));
-    x = x < -150.0f ? -150.0f : x;
-    const float n = rintf(x * HI);
-    const float f = __builtin_fmaf(x, LO, __builtin_fmaf(x, HI, -n));
-    return ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, HI, x * LO));
 }
 
-// ln(s) to about 4e-8, s a finite sum of at least 1: the power of two apart, in fp64 (s not finite or 0: as logf has it)
-__device__ static inline double tn_ln(float s) {
-    if (!(s >= 0.5f && s < 3e38f)) return (double)logf(s);
-    const int n = (int)((__float_as_uint(s) - 0x3f3504f3u) >> 23) - (s < 0.70710678f ? 512 : 0);      // s = 2^n f, f in [sqrt(1/2), sqrt(2))
-    const float f = __uint_as_float(__float_as_uint(s) - ((unsigned)n << 23));
-    return (double)n * 0.69314718055994530942 + (double)log1pf(f - 1.0f);
+// ln(s) to 1e-9, s > 0 (NaN: NaN).  s = 2^k f, f in [sqrt(1/2), sqrt(2)), z = (f - 1) / (f + 1):
+// ln f = 2 z (1 + z^2 / 3 + z^4 / 5 + ...), the bracket's sum, below 0.01, in fp32
+__device__ static inline double tn_ln(double s) {
+    double f = __builtin_amdgcn_frexp_mant(s);
+    int k = __builtin_amdgcn_frexp_exp(s);
+    if (f < 0.70710678118654752440) { f += f; --k; }
+    const double num = f - 1.0, den = f + 1.0, r = (double)__builtin_amdgcn_rcpf((float)den), z0 = num * r;
+    const double z = __builtin_fma(r, __builtin_fma(-z0, den, num), z0);
+    const float w = (float)z * (float)z;
+    float p = 1.0f / 11.0f;
+    p = __builtin_fmaf(p, w, 1.0f / 9.0f);
+    p = __builtin_fmaf(p, w, 1.0f / 7.0f);
+    p = __builtin_fmaf(p, w, 1.0f / 5.0f);
+    p = __builtin_fmaf(p, w, 1.0f / 3.0f);
+    return __builtin_fma((double)k, 0.69314718055994530942, __builtin_fma(2.0 * z, (double)(p * w), 2.0 * z));
 }
 
-// max and sum over the TPR threads of a row: the running pair of a softmax, merged
-__device__ static inline void tn_merge(float& m, float& s, float m2, float s2) {
-    const float top = fmaxf(m, m2);
-    // equal (also both -inf): no exponent of a difference of infinities
-    s = (m == top ? s : s * tn_exp<true>(m - top)) + (m2 == top ? s2 : s2 * tn_exp<true>(m2 - top));
-    m = top;
-}
+// The TPR threads' running pairs (largest value, sum of exponentials below it) become the row's, in every one of them: the
+// largest first, so that each sum is scaled once.
 template <int TPR>
-__device__ static inline void tn_row_merge(float& m, float& s, float* lds) {
+__device__ static inline void tn_row_merge(float& m, double& s, float* lds_m, double* lds_s) {
+    if (TPR == 1) return;
+    float top = m;
 #pragma unroll
-    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) {
-        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
-        tn_merge(m, s, m2, s2);
-    }
+    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     if (TPR > 64) {
-        constexpr int NW = TPR / 64;
+        if ((threadIdx.x & 63) == 0) lds_m[threadIdx.x >> 6] = top;
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) { lds[(threadIdx.x >> 6) * 2] = m; lds[(threadIdx.x >> 6) * 2 + 1] = s; }
-        __syncthreads();
-        m = lds[0]; s = lds[1];
+        top = lds_m[0];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) tn_merge(m, s, lds[2 * w], lds[2 * w + 1]);
+        for (int w = 1; w < TPR / 64; ++w) top = fmaxf(top, lds_m[w]);
+    }
+    s *= tn_exp64(m - top);                                      // (a row of -inf alone: NaN, as its log-probability)
+    m = top;
+#pragma unroll
+    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) s += __shfl_xor(s, o, 64);
+    if (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) lds_s[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = lds_s[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) s += lds_s[w];
     }
 }
 
-// eight more values into the running pair.  NaN: the sum becomes NaN and stays it.
+// n of eight more values (N: how many at most) into the running pair.  NaN: the sum becomes NaN and stays it.  FEW: each
+// exponential and the sum in fp64; else eight are added up in fp32, which many pieces average, and the pieces in fp64.
 template <bool FEW>
-__device__ static inline void tn_add8(float& m, float& s, const float (&v)[8]) {
+__device__ static inline void tn_add8(float& m, double& s, const float (&v)[8], int n = 8) {
     float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
     top = fmaxf(top, m);
-    if (top > m) { s *= tn_exp<FEW>(m - top); m = top; }     // m = -inf: s is 0 (or NaN) before
+    if (top > m) { s *= FEW ? tn_exp64(m - top) : (double)tn_exp(m - top); m = top; }     // m = -inf: s is 0 (or NaN) before
     const float base = m == -__builtin_inff() ? 0.0f : m;                            // all -inf so far: exp(-inf) = 0
-    float a = 0.0f, b = 0.0f;
+    if (FEW) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        a += tn_exp<FEW>(v[i] - base);
-        b += tn_exp<FEW>(v[i + 1] - base);
+        for (int i = 0; i < 8; ++i) {
+            if (i >= n) break;
+            s += tn_exp64(v[i] - base);
+        }
+    } else {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            a += tn_exp(v[i] - base);
+            b += tn_exp(v[i + 1] - base);
+        }
+        s += (double)(a + b);
     }
-    s += a + b;
 }
 
 // MODE 0: row statistics (and the policy's per-row terms where T.old_logp is given)
@@ -243,7 +278,8 @@ template <int DT, int TPR, int MODE, int PIECES = 4>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     constexpr int RPB = (TPR < 256 ? 256 : TPR) / TPR;
     constexpr int RPW = TPR < 64 ? 64 / TPR : 1;
-    __shared__ float lds[2 * (TPR < 64 ? 1 : TPR / 64)];
+    __shared__ float lds_m[TPR < 64 ? 1 : TPR / 64];
+    __shared__ double lds_s[TPR < 64 ? 1 : TPR / 64];
     const int t = threadIdx.x % TPR;
     const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (TPR > 1 && TPR <= 64 && r >= T.R) return;                // (TPR > 64: one row per block, none too many)
@@ -258,7 +294,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
     const bool counts = r < T.R && tn_counts(T, r, a);
     constexpr int KEEP = MODE == 1 ? 1 : TPR == 1 ? PIECES : MODE == 2 ? TN_KEEP(DT) : 1;
     eh_raw8<DT> keep[KEEP];
-    float m = -__builtin_inff(), s = 0.0f, inv = 0.0f;
+    float m = -__builtin_inff(), inv = 0.0f;
+    double s = 0.0;
     float coef = 0.0f;
     // Pieces of eight values, all whole: the last one of a row ends with it and begins inside the one before, those values are
     // left out of the sum and their gradient is written twice, to the same bits.  (8 classes or less: one piece, value by value.)
@@ -298,9 +335,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
                     add(v, c);
                 }
             } else {
-                tn_add8<true>(m, s, only);
+                tn_add8<true>(m, s, only, C);
             }
-            tn_row_merge<TPR>(m, s, lds);                         // (a row counts for all of its threads or none)
+            tn_row_merge<TPR>(m, s, lds_m, lds_s);                         // (a row counts for all of its threads or none)
         }
         double logp = 0.0;
         float d = 0.0f, term = 0.0f, kl = 0.0f;
@@ -310,7 +347,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
         if (counts) {
             const float xa = (float)row[a];
             logp = (double)xa - (double)m - tn_ln(s);
-            inv = 1.0f / s;
+            const float s32 = (float)s;
+            inv = 1.0f / s32;
+            inv = __builtin_fmaf(-inv * inv, (float)(s - (double)s32), inv);
             if (T.old_logp) {
                 if (TPR > 1) seq = tn_wave_seq<RPW>(T.seq_ptr, T.S, r);
                 d = tn_policy(T, r, seq, logp, old, ref, term, kl, cut);
