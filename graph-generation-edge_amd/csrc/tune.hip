@@ -85,8 +85,10 @@ __device__ static inline double tn_scale(const tn_rows& T, int seq) {
     return T.scale ? T.scale[seq] : T.weight ? (double)T.weight[seq] : T.each;
 }
 
-// exp(d) - 1 - d, to a few ulp: its series (d^2 / 2 + ...; the term after the last is below 2^-25 of the first) near 0
-__device__ static inline float tn_kl(float d) {
+// exp(d) - 1 - d and its derivative exp(d) - 1, to a few ulp: near 0 the series (d^2 / 2 + ...; the term after the last is
+// below 2^-25 of the first), which d added to is no cancellation; else each by itself, so that a large -d is not rounded into
+// the derivative and an infinite one (a class that the reference forbids) leaves it -1
+__device__ static inline float tn_kl(float d, float& slope) {
     if (fabsf(d) < 1.0f) {
         float s = 1.0f / 479001600.0f;
         s = s * d + 1.0f / 39916800.0f;
@@ -99,9 +101,13 @@ __device__ static inline float tn_kl(float d) {
         s = s * d + 1.0f / 24.0f;
         s = s * d + 1.0f / 6.0f;
         s = s * d + 0.5f;
-        return s * d * d;
+        s *= d * d;
+        slope = s + d;
+        return s;
     }
-    return d > 80.0f ? expf(d) : expf(d) - 1.0f - d;             // (an infinite gap is not NaN)
+    const float e = expf(d);
+    slope = e - 1.0f;
+    return d > 80.0f ? e : slope - d;                            // (an infinite gap is not NaN)
 }
 
 // the policy terms of one counted row; returns d term / d logp
@@ -116,9 +122,12 @@ __device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, d
     kl = 0.0f;
     if (T.ref) {
         const float gap = (float)((double)ref - logp);
-        kl = tn_kl(gap);
-        term += T.kl_coef * kl;
-        d -= T.kl_coef * (kl + gap);                             // exp(gap) - 1
+        float slope;
+        kl = tn_kl(gap, slope);
+        if (T.kl_coef != 0.0f) {                                 // (only watched: an infinite or NaN kl stays out of loss and gradient)
+            term += T.kl_coef * kl;
+            d -= T.kl_coef * slope;
+        }
     }
     return d;
 }

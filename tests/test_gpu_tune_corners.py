@@ -1,0 +1,72 @@
+"""GPU: values at which the losses' formulas (edgehip.tune) are finite although a part of them is not.
+
+Gradients are coef (onehot - p).  Tolerance: coef is made of A rho and kl_coef (exp(gap) - 1), each off by at most 16 half steps of
+fp32 (the log-probability's 2^-24, two exponentials', their products'), p by as many: 32 x 2^-24 of the sizes."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_tune import logp64, make, policy64
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+INF = float('inf')
+
+
+def policy(s, ref, kl_coef, mean=True, adv=None, old=None):
+    """Both forms against autograd of the formula in fp64 (kl_coef 0: without the term); returns the one-pass form."""
+    import edgehip
+    s = dict(s, adv=s['adv'] if adv is None else adv, old=s['old'] if old is None else old)
+    x = s['x'].double().requires_grad_(True)
+    lp = logp64(s, x)
+    loss, _, clipped, A, rho = policy64(s, lp, s['adv'], (0.2, 0.3), kl_coef, ref if kl_coef else None, mean)
+    S = len(loss)
+    (want,) = torch.autograd.grad(loss.sum() / S, x)
+    assert bool(torch.isfinite(want).all())
+    with torch.no_grad():
+        gap = ref.double() - lp
+        n = torch.stack([s['counts'][a:b].sum() for a, b in zip(s['ptr'].tolist(), s['ptr'].tolist()[1:])]).clamp(min=1) if mean else torch.ones(S, device='cuda')
+        own = torch.repeat_interleave(torch.arange(S, device='cuda'), s['ptr'][1:] - s['ptr'][:-1])
+        size = A.abs() * rho + (kl_coef * (torch.exp(gap) + 1) if kl_coef else 0.0)      # (of what the formula has: no term with kl_coef 0)
+        size = torch.where(s['counts'], size / (n[own] * S), 0.0)
+        p = torch.softmax(torch.where(s['counts'][:, None], s['x'].double(), 0.0), 1)
+        hot = torch.zeros_like(p).scatter_(1, s['taken'].clamp(0, p.shape[1] - 1)[:, None], 1.0)
+        tol = 32 * U * size[:, None] * (p + hot) + 1e-30
+    kw = dict(ref_logp=ref, mask=s['mask'], clip=(0.2, 0.3), kl_coef=kl_coef, reduce='mean' if mean else 'sum')
+    r = edgehip.policy_loss_grad(s['x'], s['taken'], s['old'], s['adv'], s['ptr'], **kw)
+    leaf = s['x'].clone().requires_grad_(True)
+    f = edgehip.policy_loss(leaf, s['taken'], s['old'], s['adv'], s['ptr'], **kw)
+    (g,) = torch.autograd.grad(f.loss.mean(), leaf)
+    for got in (r.dlogits, g):
+        assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+    for got in (r.loss, f.loss):
+        assert torch.equal(torch.isinf(got), torch.isinf(loss)) and not bool(got.isnan().any())
+        fin = torch.isfinite(loss)
+        assert bool(((got.double() - loss).abs()[fin] <= 1e-5 * (1 + loss.abs()[fin])).all())
+    assert torch.equal(r.clipped.cpu().long(), clipped) and torch.equal(f.clipped, r.clipped)
+    return r
+
+
+@pytest.mark.parametrize('classes', [2, 5, 40, 300])
+@pytest.mark.parametrize('mean', [True, False])
+def test_a_class_the_reference_forbids(classes, mean):
+    """ref_logp = -inf where the class was taken all the same: the loss is infinite, its derivative is not; with kl_coef 0
+    the term is only reported.  Finite gaps far below zero: exp(gap) - 1 is -1 to the last bit."""
+    s = make(90, classes, 3, seed=classes, masked=classes != 5)
+    live = s['counts'].nonzero()[:, 0]
+    for gap in (-INF, -1e30, -1e6, -1000.0, -60.0):
+        ref = s['ref'].clone()
+        ref[live[4]] = gap
+        ref[live[-3]] = gap
+        r = policy(s, ref, 0.1, mean)
+        assert int(torch.isinf(r.loss).sum()) == (0 if math.isfinite(gap) else len({int((s['ptr'][1:] <= int(live[k])).sum()) for k in (4, -3)}))
+        r = policy(s, ref, 0.0, mean)
+        assert bool(torch.isfinite(r.loss).all()) and bool((r.kl[:1] >= 0).all())
+        if gap == -INF:
+            assert bool(torch.isinf(r.kl).any())
+    ref = s['ref'].clone()
+    ref[live[4]] = float('nan')                                  # only watched: in kl alone
+    r = policy(s, ref, 0.0, mean)
+    assert bool(r.kl.isnan().any())
