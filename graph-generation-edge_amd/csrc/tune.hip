@@ -38,13 +38,13 @@ struct tn_rows {
     // policy
     const float *old_logp, *adv, *ref;
     int adv_per_row;
-    float kl_coef, lo, hi;              // 1 - lo, 1 + hi
+    double kl_coef, lo, hi;             // 1 - lo, 1 + hi
     double ln_lo, ln_hi;                // their logarithms
     // per row
     float* logp;                        // log-probability (0 where the row does not count)
     double* logp64;                     // the same, for sums whose differences matter
     float* rowstat;                     // [R][2] max and 1 / sum
-    float* term; float* kl; float* dterm; uint8_t* clipped;
+    double* term; float* kl; float* dterm; uint8_t* clipped;
     // per sequence
     const double* scale;                // factor of dterm in the gradient; NULL: weight[s], or each
     const float* weight; double each;
@@ -110,23 +110,46 @@ __device__ static inline float tn_kl(float d, float& slope) {
     return d > 80.0f ? e : slope - d;                            // (an infinite gap is not NaN)
 }
 
-// the policy terms of one counted row; returns d term / d logp
-__device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, double logp, float old, float ref, float& term, float& kl, bool& cut) {
+// e^x, x <= 700 or NaN (below -150: e^-150), in fp64 to 3.5e-8 (rms 6e-9, mean below 2e-10).  e^x = 2^n (1 + q): n = rint(x log2 e), r = x - n ln 2, ln 2
+// as 16 bits (n times them is exact) and the rest; q = e^r - 1 = r + r^2 P(r) in fp32, where its rounding is at most 2^-26; P
+// has the smallest largest error over |r| <= ln 2 / 2, 5e-10.  A row of few classes has no many terms to average over and a
+// preference's margin is the difference of sums over many such rows: rounded to fp32 and added up there, a row's
+// log-probability was off by 3e-8 to 7e-8, all margins by that times the root of their rows and more.
+__device__ static inline double tn_exp64(float x) {
+    x = x < -150.0f ? -150.0f : x;                               // (-inf; NaN stays)
+    const float t = __builtin_fmaf(x, 1.44269504f, 12582912.0f), n = t - 12582912.0f;     // n in t's last bits
+    const float r1 = __builtin_fmaf(n, -0.693145751953125f, x), c = n * -1.42860682e-6f, r = r1 + c;
+    float p = 0.00020303126f;
+    p = __builtin_fmaf(p, r, 0.001393498f);
+    p = __builtin_fmaf(p, r, 0.008332706f);
+    p = __builtin_fmaf(p, r, 0.04166643f);
+    p = __builtin_fmaf(p, r, 0.16666669f);
+    p = __builtin_fmaf(p, r, 0.5f);
+    // (c not by way of r: x - n 16 bits lies on r's grid, so that c would be rounded to the same side for all x of an n)
+    const float q = r1 + __builtin_fmaf(r * r, p, c);
+    return __builtin_ldexp(1.0 + (double)q, __float_as_int(t) - 0x4b400000);
+}
+
+// The policy terms of one counted row; returns d term / d logp.  The ratio is rounded to fp32 once, its product with the
+// advantage is exact in the fp64 term (the terms of a sequence nearly cancel where its advantages sum to zero).  An advantage of 0
+// times a ratio past fp32's range is 0, times an infinite one NaN.
+__device__ static inline float tn_policy(const tn_rows& T, int64_t r, int seq, double logp, float old, float ref, double& term, float& kl, bool& cut) {
     const float A = T.adv[T.adv_per_row ? r : seq];
     const double gain = logp - (double)old;
-    const float rho = expf((float)gain);
+    const float gain32 = (float)gain;
+    const float rho = gain > 700.0 ? __builtin_inff() : gain < -700.0 ? 0.0f : (float)(tn_exp64(gain32) * (1.0 + (gain - (double)gain32)));
     cut = A > 0.0f ? gain > T.ln_hi : (A < 0.0f && gain < T.ln_lo);
-    const float bound = A > 0.0f ? T.hi : T.lo;
-    term = -A * (cut ? bound : rho);
-    float d = cut ? 0.0f : -A * rho;
+    const double bound = A > 0.0f ? T.hi : T.lo, gained = A == 0.0f && gain < (double)__builtin_inff() ? 0.0 : (double)A * (double)rho;
+    term = cut ? -(double)A * bound : -gained;
+    float d = cut ? 0.0f : (float)-gained;
     kl = 0.0f;
     if (T.ref) {
         const float gap = (float)((double)ref - logp);
         float slope;
         kl = tn_kl(gap, slope);
-        if (T.kl_coef != 0.0f) {                                 // (only watched: an infinite or NaN kl stays out of loss and gradient)
-            term += T.kl_coef * kl;
-            d -= T.kl_coef * slope;
+        if (T.kl_coef != 0.0) {                                  // (only watched: an infinite or NaN kl stays out of loss and gradient)
+            term += T.kl_coef * (double)kl;
+            d -= (float)T.kl_coef * slope;
         }
     }
     return d;
@@ -183,26 +206,7 @@ __device__ static inline void tn_wave_part(double (&v)[WHAT == 1 ? 2 : 1], bool 
     }
 }
 
-// e^x, x <= 0 or NaN, in fp64 to 3.5e-8 (rms 6e-9, mean below 2e-10).  e^x = 2^n (1 + q): n = rint(x log2 e), r = x - n ln 2, ln 2
-// as 16 bits (n times them is exact) and the rest; q = e^r - 1 = r + r^2 P(r) in fp32, where its rounding is at most 2^-26; P
-// has the smallest largest error over |r| <= ln 2 / 2, 5e-10.  A row of few classes has no many terms to average over and a
-// preference's margin is the difference of sums over many such rows: rounded to fp32 and added up there, a row's
-// log-probability was off by 3e-8 to 7e-8, all margins by that times the root of their rows and more.
-__device__ static inline double tn_exp64(float x) {
-    x = x < -150.0f ? -150.0f : x;                               // (-inf; NaN stays)
-    const float t = __builtin_fmaf(x, 1.44269504f, 12582912.0f), n = t - 12582912.0f;     // n in t's last bits
-    const float r1 = __builtin_fmaf(n, -0.693145751953125f, x), c = n * -1.42860682e-6f, r = r1 + c;
-    float p = 0.00020303126f;
-    p = __builtin_fmaf(p, r, 0.001393498f);
-    p = __builtin_fmaf(p, r, 0.008332706f);
-    p = __builtin_fmaf(p, r, 0.04166643f);
-    p = __builtin_fmaf(p, r, 0.16666669f);
-    p = __builtin_fmaf(p, r, 0.5f);
-    // (c not by way of r: x - n 16 bits lies on r's grid, so that c would be rounded to the same side for all x of an n)
-    const float q = r1 + __builtin_fmaf(r * r, p, c);
-    return __builtin_ldexp(1.0 + (double)q, __float_as_int(t) - 0x4b400000);
-}
-// The same in fp32 by the hardware's power of two, for rows of many classes.  The fp32 constant log2(e) alone is 1.3e-8 off:
+// e^x in fp32 by the hardware's power of two, for rows of many classes.  The fp32 constant log2(e) alone is 1.3e-8 off:
 // every term of a row would be off to the same side by that times |x|.  With the constant's second part the error of a term
 // is that of rounding x log2(e), to either side, and the instruction's own (mean -3e-9).
 __device__ static inline float tn_exp(float x) {
@@ -349,7 +353,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
             tn_row_merge<TPR>(m, s, lds_m, lds_s);                         // (a row counts for all of its threads or none)
         }
         double logp = 0.0;
-        float d = 0.0f, term = 0.0f, kl = 0.0f;
+        double term = 0.0;
+        float d = 0.0f, kl = 0.0f;
         bool cut = false;
         int seq = -1;
         if (TPR == 1 && T.old_logp) seq = tn_lane_seq(T, r);
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_tn_rows(tn_rows T) {
             }
         }
         if (TPR == 1 && T.old_logp) {
-            double v[2] = {(double)term, (double)kl};
+            double v[2] = {term, (double)kl};
             tn_wave_part<1>(v, cut, counts, seq, r / TN_WAVE, T.part);
         }
         if (TPR == 1 && r >= T.R) return;
@@ -608,8 +613,8 @@ static tn_rows tn_fill(const edgehip_logit_rows* Q) {
     T.taken = Q->taken; T.mask = Q->mask; T.seq_ptr = Q->seq_ptr; T.S = Q->num_seqs;
     return T;
 }
-// workspace: [S] fp64 scales, [chunks + S][4] fp64 partials, per row fp32 term, kl, dterm (or stat) and a byte
-struct tn_ws { double *scale, *part, *logp; float *term, *kl, *dterm, *stat; uint8_t* clipped; size_t bytes; };
+// workspace: [S] fp64 scales, [chunks + S][4] fp64 partials, per row fp64 term, log-probability, fp32 kl, dterm, stat and a byte
+struct tn_ws { double *scale, *part, *term, *logp; float *kl, *dterm, *stat; uint8_t* clipped; size_t bytes; };
 static tn_ws tn_layout(const edgehip_logit_rows* Q, void* ws) {
     tn_ws W;
     const size_t R = (size_t)Q->rows, S = (size_t)Q->num_seqs, chunks = (R + TN_WAVE - 1) / TN_WAVE;
@@ -618,7 +623,7 @@ static tn_ws tn_layout(const edgehip_logit_rows* Q, void* ws) {
     auto take = [&](size_t n) { char* q = p + o; o += (n + 15) & ~(size_t)15; return q; };
     W.scale = (double*)take(S * 8);
     W.part = (double*)take((chunks + S) * 32);
-    W.term = (float*)take(R * 4);
+    W.term = (double*)take(R * 8);
     W.kl = (float*)take(R * 4);
     W.dterm = (float*)take(R * 4);
     W.logp = (double*)take(R * 8);
@@ -658,7 +663,7 @@ static int tn_policy_args(const edgehip_logit_rows* Q, const edgehip_policy* O, 
     W = tn_layout(Q, ws);
     T = tn_fill(Q);
     T.old_logp = O->old_logp; T.adv = O->advantage; T.ref = O->ref_logp; T.adv_per_row = O->advantage_per_row;
-    T.kl_coef = (float)O->kl_coef; T.lo = (float)(1.0 - O->clip_lo); T.hi = (float)(1.0 + O->clip_hi);
+    T.kl_coef = O->kl_coef; T.lo = 1.0 - O->clip_lo; T.hi = 1.0 + O->clip_hi;
     T.ln_lo = O->clip_lo < 1.0 ? log1p(-O->clip_lo) : -HUGE_VAL; T.ln_hi = log1p(O->clip_hi);
     T.term = W.term; T.kl = W.kl; T.clipped = W.clipped; T.part = W.part;
     T.weight = O->weight; T.each = 1.0 / (double)Q->num_seqs;

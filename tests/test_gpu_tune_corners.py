@@ -70,3 +70,16 @@ def test_a_class_the_reference_forbids(classes, mean):
     ref[live[4]] = float('nan')                                  # only watched: in kl alone
     r = policy(s, ref, 0.0, mean)
     assert bool(r.kl.isnan().any())
+
+
+@pytest.mark.parametrize('classes', [3, 40, 300])
+def test_an_advantage_of_nothing_and_a_ratio_past_the_range(classes):
+    """old_logp so low that exp(logp - old_logp) leaves fp32: 0 where the advantage is 0, bounded where the clip binds."""
+    s = make(80, classes, 4, seed=classes)
+    live = s['counts'].nonzero()[:, 0]
+    for old in (-120.0, -500.0):
+        adv = torch.tensor([0.0, 1.5, 0.0, 0.25], device='cuda')
+        far = s['old'].clone()
+        far[live[::3]] = old
+        r = policy(s, s['ref'], 0.1, adv=adv, old=far)
+        assert bool(torch.isfinite(r.loss).all())
