@@ -540,7 +540,9 @@ __global__ __launch_bounds__(DIRECT ? 1024 : 256) void k_tn_pref_final(tn_final 
     double loss, d;
     if (F.kind == EDGEHIP_PREFER_SIGMOID) {
         const double x = F.beta * margin, w = exp(-fabs(x));
-        loss = log1p(w) + (x < 0.0 ? -x : 0.0) + F.smooth * x;                   // -ln sigmoid(x), smoothed
+        // -ln sigmoid(x), smoothed: ln(1 + e^-|x|) and (1 - smooth) |x| below 0, smooth |x| above (no smooth, no term: a margin may
+        // be infinite, where a class that may not be taken was)
+        loss = log1p(w) + (x < 0.0 ? (F.smooth - 1.0) * x : F.smooth > 0.0 ? F.smooth * x : 0.0);
         d = F.beta * (F.smooth - (x >= 0.0 ? w : 1.0) / (1.0 + w));               // smooth - sigmoid(-x)
     } else {
         const double off = margin - 0.5 / F.beta;

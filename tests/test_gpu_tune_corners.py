@@ -83,3 +83,35 @@ def test_an_advantage_of_nothing_and_a_ratio_past_the_range(classes):
         far[live[::3]] = old
         r = policy(s, s['ref'], 0.1, adv=adv, old=far)
         assert bool(torch.isfinite(r.loss).all())
+
+
+@pytest.mark.parametrize('smooth', [0.0, 0.1])
+@pytest.mark.parametrize('mean', [False, True])
+@pytest.mark.parametrize('classes', [3, 100])
+def test_margins_without_end(classes, mean, smooth):
+    """A taken class of logit -inf: the preferred sequence's margin is -inf (loss inf), the other's +inf (loss 0, or inf where
+    smoothing asks for it), and the gradient is that of the formula's limit: beta (smooth - sigmoid(-x)), x = -inf, inf, 1.7."""
+    import edgehip
+    g = torch.Generator(device='cuda').manual_seed(classes)
+    x = torch.randn(12, classes, generator=g, device='cuda')
+    taken = torch.randint(0, classes, (12,), generator=g, device='cuda')
+    for row in (1, 8):                                           # in sequence 0 (preferred) and in 4 (the other of pair 1)
+        x[row, taken[row]] = -INF
+    ptr = torch.arange(0, 13, 2, device='cuda')
+    beta = 0.3
+    leaf = x.clone().requires_grad_(True)
+    f = edgehip.preference_loss(leaf, taken, ptr, beta=beta, label_smoothing=smooth, reduce='mean' if mean else 'sum')
+    r = edgehip.preference_loss_grad(x, taken, ptr, beta=beta, label_smoothing=smooth, reduce='mean' if mean else 'sum')
+    assert torch.equal(f.loss, r.loss) and torch.equal(f.margin, r.margin)
+    assert r.margin[:2].tolist() == [-INF, INF] and r.loss[:2].tolist() == [INF, INF if smooth else 0.0]
+    assert bool(torch.isfinite(r.loss[2]))
+    (grad,) = torch.autograd.grad(f.loss.mean(), leaf)
+    m = beta * r.margin.double()
+    slope = beta * (smooth - torch.sigmoid(-m)) / 3 / (2 if mean else 1)
+    coef = torch.cat([slope, -slope]).repeat_interleave(2)[:, None]
+    hot = torch.zeros_like(x, dtype=torch.float64).scatter_(1, taken[:, None], 1.0)
+    p = torch.softmax(x.double(), 1)
+    want = coef * (hot - p)
+    for got in (grad, r.dlogits):
+        # coef: the margin's 2^-24 (its size, 6 at most, in units of 1) and four roundings; p: eight
+        assert bool(((got.double() - want).abs() <= 32 * U * coef.abs() * (hot + p) + 1e-30).all())
