@@ -28,7 +28,6 @@
 // policy loss and gradient: four threads a row 105 / 102 us, one 62 / 70 us; 10^6 x 48 fp32: 128 us, 147 us).  Only written
 // (preference loss and gradient, 10^6 x 24 / 10^6 x 32 bf16: one 71 / 100 us, four 60 / 64 us): 16 classes.
 #define TN_ALONE(DT, MODE) ((MODE) == 1 ? 16 : (DT) != EDGEHIP_F32 ? 64 : 32)
-#define TN_LOG2E 1.44269504088896341f
 
 struct tn_rows {
     const void* logits; int64_t ld;     // values from one row to the next
@@ -206,7 +205,7 @@ __device__ static inline void tn_wave_part(double (&v)[WHAT == 1 ? 2 : 1], bool 
     }
 }
 
-// e^x in fp32 by the hardware's power of two, for rows of many classes.  The fp32 constant log2(e) alone is 1.3e-8 off:
+// e^x in fp32 by the hardware's power of two, for the sums of rows of many classes and for every value of a gradient.  The fp32 constant log2(e) alone is 1.3e-8 off:
 // every term of a row would be off to the same side by that times |x|.  With the constant's second part the error of a term
 // is that of rounding x log2(e), to either side, and the instruction's own (mean -3e-9).
 __device__ static inline float tn_exp(float x) {
@@ -415,7 +414,7 @@ __global__ __launch_bounds__((TPR < 256 ? 256 : TPR), TN_WAVES(TPR, MODE)) void 
                         for (int i = 0; i < 8; ++i) v[i] = only[i];
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = f * __builtin_amdgcn_exp2f((v[i] - m) * TN_LOG2E);
+                    for (int i = 0; i < 8; ++i) v[i] = f * tn_exp(v[i] - m);
                     if (a >= c && a < c + 8) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) if (a == c + i) v[i] += coef;
