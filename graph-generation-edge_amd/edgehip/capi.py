@@ -278,6 +278,16 @@ def on_gpu(what, t):
         raise ValueError(f'{what}: the tensors must be on a GPU (there is no CPU path), got {t.device}')
 
 
+def no_tangents(what, *tensors):
+    """Forward-mode derivatives: there are none, and a tensor's tangent must not get lost on the way past autograd."""
+    from torch.autograd import forward_ad
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'{what}: no forward-mode derivative (gradients are made by its backward pass)')
+
+
 class on_device_of:
     """with on_device_of(t) as s: t's GPU is current and s is its current stream."""
     __slots__ = ('index', 'before')

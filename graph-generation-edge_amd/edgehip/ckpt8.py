@@ -162,6 +162,7 @@ class _Act8(Function):
 
 def act8(x, kind='silu'):
     """act(x), keeping x in 8 bits for the backward pass."""
+    capi.no_tangents('act8', x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Act8.apply(x, kind)
     return act8_fwd(x, kind)[0]

@@ -1,0 +1,25 @@
+"""CPU: calls of the operators for deeper networks and tuning (edgehip.block, ckpt8, tune) that are refused, or taken, before any
+kernel runs."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+vec = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    """A tangent is never lost silently, whichever input has it; without one the call goes on to its other checks."""
+    import edgehip
+    h, z, w, g = vec(6, 8), vec(6, 8), vec(8), vec(6, 8)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for args, kw in (((dual(h), z), {}), ((h, dual(z)), {}), ((h, z), dict(w_pre=dual(w))), ((h, z), dict(w_post=dual(w))),
+                         ((h, z), dict(gate=dual(g))), ((h, z), dict(b_pre=dual(w), kind='layer')), ((h, z), dict(b_post=dual(w), kind='layer'))):
+            with pytest.raises(NotImplementedError, match='gate_norm: no forward-mode derivative'):
+                edgehip.gate_norm(*args, **kw)
+        with pytest.raises(NotImplementedError, match='act8: no forward-mode derivative'):
+            edgehip.act8(dual(h))
+        for f in (lambda: edgehip.gate_norm(h, z, w_pre=w), lambda: edgehip.act8(h)):
+            with pytest.raises(ValueError, match='on a GPU'):
+                f()
