@@ -32,7 +32,8 @@
 struct tn_rows {
     const void* logits; int64_t ld;     // values from one row to the next
     int64_t R; int C;
-    const int64_t* taken; const uint8_t* mask;
+    const void* taken; int taken8;      // int64, or uint8
+    const uint8_t* mask;
     const int64_t* seq_ptr; int S;
     // policy
     const float *old_logp, *adv, *ref;
@@ -52,7 +53,7 @@ struct tn_rows {
 };
 
 __device__ static inline bool tn_counts(const tn_rows& T, int64_t r, int64_t& a) {
-    a = T.taken[r];                                              // (all requests at once, no branch between them)
+    a = T.taken8 ? (int64_t)static_cast<const uint8_t*>(T.taken)[r] : static_cast<const int64_t*>(T.taken)[r];      // (all requests at once, no branch between them)
     bool on = (a >= 0) & (a < T.C);
     if (T.mask) on &= T.mask[r] != 0;
     if (T.seq_ptr) on &= (r >= T.seq_ptr[0]) & (r < T.seq_ptr[T.S]);
@@ -608,6 +609,7 @@ static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
 static int tn_check(const edgehip_logit_rows* Q, bool seqs = true) {
     EH_CHECK_ARG(Q && eh_dtype_ok(Q->dtype) && Q->rows >= 0 && Q->classes >= 1);
     EH_CHECK_ARG(seqs ? Q->seq_ptr && Q->num_seqs >= 1 : (Q->seq_ptr != nullptr) == (Q->num_seqs >= 1) && Q->num_seqs >= 0);
+    EH_CHECK_ARG(Q->taken_type == EDGEHIP_TAKEN_I64 || Q->taken_type == EDGEHIP_TAKEN_U8);
     EH_CHECK_ARG(Q->rows == 0 || (Q->logits && Q->taken && Q->row_stride >= Q->classes));
     if (Q->rows > (((int64_t)1 << 31) - 1) || Q->num_seqs > (1 << 30) || Q->classes > (1 << 30)) return EDGEHIP_ERR_TOO_LARGE;
     return EDGEHIP_OK;
@@ -615,7 +617,7 @@ static int tn_check(const edgehip_logit_rows* Q, bool seqs = true) {
 static tn_rows tn_fill(const edgehip_logit_rows* Q) {
     tn_rows T = {};
     T.logits = Q->logits; T.ld = Q->row_stride; T.R = Q->rows; T.C = Q->classes;
-    T.taken = Q->taken; T.mask = Q->mask; T.seq_ptr = Q->seq_ptr; T.S = Q->num_seqs;
+    T.taken = Q->taken; T.taken8 = Q->taken_type == EDGEHIP_TAKEN_U8; T.mask = Q->mask; T.seq_ptr = Q->seq_ptr; T.S = Q->num_seqs;
     return T;
 }
 // workspace: [S] fp64 scales, [chunks + S][4] fp64 partials, per row fp64 term, log-probability, fp32 kl, dterm, stat and a byte

@@ -71,7 +71,7 @@ class GateNorm(C.Structure):
 
 class LogitRows(C.Structure):
     _fields_ = [('rows', C.c_int64), ('row_stride', C.c_int64), ('classes', C.c_int32), ('dtype', C.c_int32),
-                ('num_seqs', C.c_int32), ('reserved', C.c_int32), ('logits', vp), ('taken', vp), ('mask', vp), ('seq_ptr', vp)]
+                ('num_seqs', C.c_int32), ('taken_type', C.c_int32), ('logits', vp), ('taken', vp), ('mask', vp), ('seq_ptr', vp)]
 
 
 class Policy(C.Structure):

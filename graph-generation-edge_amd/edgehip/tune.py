@@ -1,11 +1,11 @@
 """tune.py - losses over rows of logits that tune a trained model (csrc/tune.hip): a clipped policy loss with a KL term and
 a paired preference loss, each with its gradient.
 
-A row of logits is one decision (a token; an active pair of a graph, classes 0 / 1), `taken` what was chosen there, and
-the rows of one sequence (an answer; a graph) are consecutive: sequence s is rows seq_ptr[s] .. seq_ptr[s+1]-1, ascending
-from 0, empty ones allowed (`aptr` of the active pairs is a seq_ptr).  A row counts unless its mask is False, its
-`taken` lies outside the classes (-100, say) or it lies in no sequence; what stands in the logits of the others does not
-matter, and their gradient is 0.
+A row of logits is one decision (a token; an active pair of a graph, classes 0 / 1), `taken` what was chosen there (int64,
+or uint8 as the sampler's bits are), and the rows of one sequence (an answer; a graph) are consecutive: sequence s is rows
+seq_ptr[s] .. seq_ptr[s+1]-1, ascending from 0, empty ones allowed (`aptr` of the active pairs is a seq_ptr).  A row counts
+unless its mask is False, its `taken` lies outside the classes (-100, say) or it lies in no sequence; what stands in the
+logits of the others does not matter, and their gradient is 0.
 
 `policy_loss` / `preference_loss` are differentiable in the logits; the `_grad` forms return the gradient of
 sum(weight * loss) at once, without a graph (`logits.backward(r.dlogits)` goes on from it)."""
@@ -49,7 +49,8 @@ def _describe(what, logits, taken, seq_ptr, mask):
     dev = logits.device
     if classes > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < classes:
         logits = logits.contiguous()
-    taken = _vector(what, 'taken', taken, rows, torch.int64, dev)
+    small = taken.dtype == torch.uint8
+    taken = _vector(what, 'taken', taken, rows, torch.uint8 if small else torch.int64, dev)
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f'{what}: mask must be bool or uint8, got {mask.dtype}')
@@ -62,6 +63,7 @@ def _describe(what, logits, taken, seq_ptr, mask):
     Q = capi.LogitRows()
     Q.rows, Q.classes, Q.dtype = rows, classes, code
     Q.row_stride = logits.stride(0) if rows > 1 else classes
+    Q.taken_type = int(small)
     Q.num_seqs = 0 if seq_ptr is None else seq_ptr.numel() - 1
     Q.logits, Q.taken, Q.mask, Q.seq_ptr = logits.data_ptr(), taken.data_ptr(), capi.ptr(mask), capi.ptr(seq_ptr)
     return Q, (logits, taken, mask, seq_ptr)

@@ -549,11 +549,13 @@ int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const int8_t* code
  * rows seq_ptr[s] .. seq_ptr[s+1]-1 (ascending from 0; the `aptr` of the active pairs is one).  A row counts if
  * mask[r] != 0 (mask NULL: every row), 0 <= taken[r] < classes and it lies in a sequence; the others have log-probability
  * 0 and gradient 0 whatever their logits hold.  dlogits is dense [rows, classes], of the logits' dtype, written whole. */
+#define EDGEHIP_TAKEN_I64 0
+#define EDGEHIP_TAKEN_U8 1               /* what edgehip_edge_resample puts out */
 typedef struct edgehip_logit_rows {
     int64_t rows, row_stride;
-    int32_t classes, dtype, num_seqs, reserved;
+    int32_t classes, dtype, num_seqs, taken_type;
     const void* logits;
-    const int64_t* taken;
+    const void* taken;                   /* [rows] int64 or uint8 */
     const uint8_t* mask;
     const int64_t* seq_ptr;              /* [num_seqs+1] */
 } edgehip_logit_rows;

@@ -115,3 +115,56 @@ def test_margins_without_end(classes, mean, smooth):
     for got in (grad, r.dlogits):
         # coef: the margin's 2^-24 (its size, 6 at most, in units of 1) and four roundings; p: eight
         assert bool(((got.double() - want).abs() <= 32 * U * coef.abs() * (hot + p) + 1e-30).all())
+
+
+@pytest.mark.parametrize('classes', [2, 9, 40, 200, 300, 9000])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_choices_of_one_byte(classes, dtype):
+    """taken as uint8: the same bits as with the same choices in int64, classes out of range among them."""
+    import edgehip
+    s = make(700, classes, 4, dtype, seed=classes)
+    small = s['taken'].clamp(min=0) % 256                        # (-100: another row's 0; 255 and the like lie outside of few classes)
+    small[5] = 255
+    small = small.to(torch.uint8)
+    for f in (lambda t: edgehip.policy_loss_grad(s['x'], t, s['old'], s['adv'], s['ptr'], ref_logp=s['ref'], mask=s['mask'], kl_coef=0.1),
+              lambda t: edgehip.preference_loss_grad(s['x'], t, s['ptr'], ref_logp=s['ref'], mask=s['mask']),
+              lambda t: edgehip.policy_loss(s['x'], t, s['old'], s['adv'], s['ptr']), lambda t: edgehip.preference_loss(s['x'], t, s['ptr']),
+              lambda t: [edgehip.row_logp(s['x'], t, s['mask'])]):
+        got, want = f(small), f(small.long())
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(got, want))
+    leaf = s['x'].clone().requires_grad_(True)
+    a, b = (torch.autograd.grad(edgehip.policy_loss(leaf, t, s['old'], s['adv'], s['ptr'], mask=s['mask']).loss.sum(), leaf)[0] for t in (small, small.long()))
+    assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+def test_the_samplers_own_decisions():
+    """A reverse step's logits and bits, as it hands them out, with `aptr` as the sequences."""
+    import numpy as np
+
+    import cases
+    import edgehip
+    import helpers as H
+    from edgehip.model import _state
+    from oracle import edge_oracle as orc
+    graphs = cases.ragged_graphs(5)
+    model = H.build_model(orc.random_tgnn_params(4), 48, cases.max_degree_of(graphs))
+    b = H.graph_batch(graphs)
+    rng, want = np.random.default_rng(1), {}
+    draw = lambda n: cases.uniforms(rng, n, 2).cuda()
+    H.set_state_from_pair_indices(b, torch.arange(0, sum(q['n'] * (q['n'] - 1) // 2 for q in graphs), 5))
+    model.p_sample(b, 9, draw(b.num_nodes), draw, None, None, want)
+    logits, bits, aptr = want['logits'], want['bits'], _state(b)['aptr']
+    assert bits.dtype == torch.uint8 and bits.numel() > 50 and int(aptr[-1]) == bits.numel()
+    old = edgehip.row_logp(logits, bits)
+    lp = torch.log_softmax(logits.double(), 1).gather(1, bits.long()[:, None])[:, 0]
+    assert bool(((old.double() - lp).abs() <= 2 * U * (1 + lp.abs())).all())
+    adv = torch.linspace(-1, 1, b.num_graphs, device='cuda')
+    r = edgehip.policy_loss_grad(logits, bits, old, adv, aptr)
+    n = (aptr[1:] - aptr[:-1]).clamp(min=1)
+    has = aptr[1:] > aptr[:-1]
+    assert bool(((r.loss + adv)[has].abs() <= 1e-6).all())       # ratio 1 everywhere
+    own = torch.repeat_interleave(torch.arange(b.num_graphs, device='cuda'), aptr[1:] - aptr[:-1])
+    hot = torch.nn.functional.one_hot(bits.long(), 2).double()
+    coef = -(adv.double() / n / b.num_graphs)[own][:, None]
+    p = torch.softmax(logits.double(), 1)
+    assert bool(((r.dlogits.double() - coef * (hot - p)).abs() <= 32 * U * coef.abs() * (hot + p) + 1e-30).all())
