@@ -161,7 +161,7 @@ static int ck_size(int64_t M, int64_t K, unsigned& KG, unsigned& ngroups) {
     EH_CHECK_ARG(M >= 0 && K >= 1);
     if (K > ((int64_t)1 << 31) - 64) return EDGEHIP_ERR_TOO_LARGE;
     const int64_t kg = (K + CK_GROUP - 1) / CK_GROUP;
-    if (M > 0 && kg > (((int64_t)1 << 31) - 1) / M) return EDGEHIP_ERR_TOO_LARGE;
+    if (M > 0 && (kg > (((int64_t)1 << 31) - 1) / M || !eh_grid_ok((M * kg + 31) / 32, 256))) return EDGEHIP_ERR_TOO_LARGE;
     KG = (unsigned)kg;
     ngroups = (unsigned)(M * kg);
     return EDGEHIP_OK;
@@ -640,7 +640,8 @@ static dw_plan dw_choose(int64_t M, int N, int K) {
 static int dw_check(int32_t dtype, int64_t M, int32_t N, int32_t K) {
     EH_CHECK_ARG(eh_dtype_ok(dtype) && M >= 0 && N >= 1 && K >= 1);
     if (N > (1 << 22) || K > (1 << 22)) return EDGEHIP_ERR_TOO_LARGE;        // offsets within 64 rows are 32 bits
-    return EDGEHIP_OK;
+    const dw_plan p = dw_choose(M, N, K);
+    return eh_grid_ok((int64_t)p.nt * p.kt, 256) ? EDGEHIP_OK : EDGEHIP_ERR_TOO_LARGE;
 }
 
 static size_t dw_floats(const dw_plan& p, int N, int K, size_t& db_at) {

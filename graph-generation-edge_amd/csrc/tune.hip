@@ -581,24 +581,37 @@ static void tn_go(const tn_rows& T, int tpr, dim3 grid, dim3 block, hipStream_t 
 }
 template <int MODE> static int tn_alone(int dtype) { return dtype == EDGEHIP_F32 ? TN_ALONE(EDGEHIP_F32, MODE) : TN_ALONE(EDGEHIP_BF16, MODE); }
 template <int MODE>
-static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
-    if (T.R == 0) return EDGEHIP_OK;
+static int tn_threads(int dtype, int C) {
     // Threads of a row: one for few classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 247 us, one
     // 36 us), else as few as can keep it whole: what is done once per row is done by all of them, and a CU has rows in
     // different phases (8192 x 32003 bf16: 1024 threads a row 382 us, 256 237 us; 10^5 x 513 bf16: 64 threads 213 us, 8
     // 72 us).
     const int per = 8 * (dtype == EDGEHIP_F32 ? TN_KEEP(EDGEHIP_F32) : TN_KEEP(EDGEHIP_BF16));
-    int tpr = 1;
-    if (T.C > tn_alone<MODE>(dtype)) {
-        // (only written: wider runs pay more where a row has more than 128 bytes; preference over 10^6 x 48 fp32: four threads
-        // 154 us, eight 135 us; over 10^6 x 33 bf16: 97 us, 107 us)
-        tpr = MODE == 1 && T.C > (dtype == EDGEHIP_F32 ? 32 : 64) ? 8 : 4;
-        while (tpr < 64 && T.C > tpr * per) tpr *= 2;
-        if (T.C > 64 * per) tpr = 256;
-        while (tpr < 1024 && T.C > tpr * per) tpr *= 2;
-    }
-    const int rpb = (tpr < 256 ? 256 : tpr) / tpr;
-    const dim3 grid((unsigned)((T.R + rpb - 1) / rpb)), block(tpr < 256 ? 256 : tpr);
+    if (C <= tn_alone<MODE>(dtype)) return 1;
+    // (only written: wider runs pay more where a row has more than 128 bytes; preference over 10^6 x 48 fp32: four threads
+    // 154 us, eight 135 us; over 10^6 x 33 bf16: 97 us, 107 us)
+    int tpr = MODE == 1 && C > (dtype == EDGEHIP_F32 ? 32 : 64) ? 8 : 4;
+    while (tpr < 64 && C > tpr * per) tpr *= 2;
+    if (C > 64 * per) tpr = 256;
+    while (tpr < 1024 && C > tpr * per) tpr *= 2;
+    return tpr;
+}
+template <int MODE>
+static int64_t tn_row_blocks(int dtype, int64_t R, int C) {
+    const int tpr = tn_threads<MODE>(dtype, C), rpb = (tpr < 256 ? 256 : tpr) / tpr;
+    return (R + rpb - 1) / rpb;
+}
+// whether a launch takes all rows: up to 2^31 - 1 of few classes, fewer with several threads a row
+template <int MODE>
+static int tn_fits(const edgehip_logit_rows* Q) {
+    const int tpr = tn_threads<MODE>(Q->dtype, Q->classes);
+    return eh_grid_ok(tn_row_blocks<MODE>(Q->dtype, Q->rows, Q->classes), tpr < 256 ? 256 : tpr) ? EDGEHIP_OK : EDGEHIP_ERR_TOO_LARGE;
+}
+template <int MODE>
+static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
+    if (T.R == 0) return EDGEHIP_OK;
+    const int tpr = tn_threads<MODE>(dtype, T.C);
+    const dim3 grid((unsigned)tn_row_blocks<MODE>(dtype, T.R, T.C)), block(tpr < 256 ? 256 : tpr);
     if (dtype == EDGEHIP_F32) tn_go<EDGEHIP_F32, MODE>(T, tpr, grid, block, s);
     else if (dtype == EDGEHIP_BF16) tn_go<EDGEHIP_BF16, MODE>(T, tpr, grid, block, s);
     else tn_go<EDGEHIP_F16, MODE>(T, tpr, grid, block, s);
@@ -606,12 +619,14 @@ static int tn_launch(int dtype, const tn_rows& T, hipStream_t s) {
     return EDGEHIP_OK;
 }
 
+#define TN_TRY(x) do { const int rc_ = (x); if (rc_ != EDGEHIP_OK) return rc_; } while (0)
 static int tn_check(const edgehip_logit_rows* Q, bool seqs = true) {
     EH_CHECK_ARG(Q && eh_dtype_ok(Q->dtype) && Q->rows >= 0 && Q->classes >= 1);
     EH_CHECK_ARG(seqs ? Q->seq_ptr && Q->num_seqs >= 1 : (Q->seq_ptr != nullptr) == (Q->num_seqs >= 1) && Q->num_seqs >= 0);
     EH_CHECK_ARG(Q->taken_type == EDGEHIP_TAKEN_I64 || Q->taken_type == EDGEHIP_TAKEN_U8);
     EH_CHECK_ARG(Q->rows == 0 || (Q->logits && Q->taken && Q->row_stride >= Q->classes));
-    if (Q->rows > (((int64_t)1 << 31) - 1) || Q->num_seqs > (1 << 30) || Q->classes > (1 << 30)) return EDGEHIP_ERR_TOO_LARGE;
+    // (sequences: a block each)
+    if (Q->rows > (((int64_t)1 << 31) - 1) || !eh_grid_ok(Q->num_seqs, 256) || Q->classes > (1 << 30)) return EDGEHIP_ERR_TOO_LARGE;
     return EDGEHIP_OK;
 }
 static tn_rows tn_fill(const edgehip_logit_rows* Q) {
@@ -651,11 +666,11 @@ static int tn_sum(const tn_rows& T, hipStream_t s) {
     return EDGEHIP_OK;
 }
 
-#define TN_TRY(x) do { const int rc_ = (x); if (rc_ != EDGEHIP_OK) return rc_; } while (0)
 
 extern "C" int edgehip_row_logp(const edgehip_logit_rows* Q, float* logp, void* stream) {
     TN_TRY(tn_check(Q, false));
     EH_CHECK_ARG(Q->rows == 0 || logp);
+    TN_TRY(tn_fits<0>(Q));
     tn_rows T = tn_fill(Q);
     T.logp = logp;
     return tn_launch<0>(Q->dtype, T, eh_stream(stream));
@@ -701,6 +716,7 @@ extern "C" int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehi
     tn_rows T; tn_final F; tn_ws W;
     TN_TRY(tn_policy_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(loss && kl && clipped);
+    TN_TRY(tn_fits<0>(Q));
     hipStream_t s = eh_stream(stream);
     T.logp = logp; T.rowstat = W.stat; T.dterm = W.dterm;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
@@ -712,6 +728,7 @@ extern "C" int edgehip_policy_loss_bwd(const edgehip_logit_rows* Q, const edgehi
     tn_rows T; tn_final F; tn_ws W;
     TN_TRY(tn_policy_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(Q->rows == 0 || dlogits);
+    TN_TRY(tn_fits<1>(Q));
     hipStream_t s = eh_stream(stream);
     if (F.mean) {                               // the partial sums of the forward, if it made some, are still in the workspace
         F.scale = W.scale;
@@ -726,6 +743,7 @@ extern "C" int edgehip_policy_loss_grad(const edgehip_logit_rows* Q, const edgeh
     tn_rows T; tn_final F; tn_ws W;
     TN_TRY(tn_policy_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(loss && kl && clipped && (Q->rows == 0 || dlogits));
+    TN_TRY(tn_fits<2>(Q));
     hipStream_t s = eh_stream(stream);
     if (F.mean) {                               // a mean needs the number of counted rows before the gradient
         if (!tn_direct(T)) TN_TRY(tn_sum<0>(T, s));
@@ -762,6 +780,7 @@ static int tn_pref_final(const tn_final& F, const tn_rows& T, hipStream_t s) {
 }
 static int tn_pref_fwd(const edgehip_logit_rows* Q, tn_rows& T, tn_final& F, tn_ws& W, float* loss, float* margin, hipStream_t s) {
     EH_CHECK_ARG(loss && margin);
+    TN_TRY(tn_fits<0>(Q));
     T.logp64 = W.logp; T.rowstat = W.stat;
     TN_TRY(tn_launch<0>(Q->dtype, T, s));
     if (!tn_direct(T)) TN_TRY(tn_sum<2>(T, s));
@@ -780,6 +799,7 @@ extern "C" int edgehip_preference_loss_grad(const edgehip_logit_rows* Q, const e
     tn_rows T; tn_final F; tn_ws W;
     TN_TRY(tn_pref_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(Q->rows == 0 || dlogits);
+    TN_TRY(tn_fits<1>(Q));
     F.scale = W.scale;
     TN_TRY(tn_pref_fwd(Q, T, F, W, loss, margin, eh_stream(stream)));
     T.logp64 = nullptr; T.scale = W.scale; T.dlogits = dlogits;
@@ -790,6 +810,7 @@ extern "C" int edgehip_preference_loss_bwd(const edgehip_logit_rows* Q, const ed
     tn_rows T; tn_final F; tn_ws W;
     TN_TRY(tn_pref_args(Q, O, T, F, W, ws, ws_bytes));
     EH_CHECK_ARG(Q->rows == 0 || dlogits);
+    TN_TRY(tn_fits<1>(Q));
     hipStream_t s = eh_stream(stream);
     F.scale = W.scale;
     T.logp64 = W.logp;                          // (what the forward left there)

@@ -16,6 +16,8 @@ typedef unsigned int eh_u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int eh_u32x2u __attribute__((ext_vector_type(2), aligned(1)));
 typedef unsigned int eh_u32x2h __attribute__((ext_vector_type(2), aligned(2)));
 
+// whether a launch takes that many threads along x (its size is a 32-bit number of threads)
+static inline int eh_grid_ok(int64_t blocks, int64_t threads) { return blocks < ((int64_t)1 << 32) / threads; }
 static inline int eh_dtype_ok(int dt) { return dt == EDGEHIP_F32 || dt == EDGEHIP_BF16 || dt == EDGEHIP_F16; }
 
 // eight raw values as they stand in memory (4 or 8 registers)

@@ -212,9 +212,13 @@ class EdgeHipError(RuntimeError):
     pass
 
 
+class EdgeHipSizeError(EdgeHipError, ValueError):
+    """An argument larger than the call takes."""
+
+
 def check(rc, what=''):
     if rc != OK:
-        raise EdgeHipError(f'{what}: {_ERR.get(rc, rc)} ({rc})')
+        raise (EdgeHipSizeError if rc == ERR_TOO_LARGE else EdgeHipError)(f'{what}: {_ERR.get(rc, rc)} ({rc})')
 
 
 MISC_EXPORTS = ('edgehip_edge_ce_loss_static_max_tiles', 'edgehip_train_set_side_stream', 'edgehip_layout_pair_tile_bound')

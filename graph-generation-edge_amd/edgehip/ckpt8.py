@@ -12,6 +12,7 @@ from . import capi
 
 lib = capi.lib
 GROUP = 64
+MAX_GROUPS = (1 << 29) - 32
 KINDS = {'silu': 1, 'mish': 2}
 _TORCH_TYPE = {capi.F32: torch.float32, capi.BF16: torch.bfloat16, capi.F16: torch.float16}
 
@@ -54,6 +55,8 @@ def _input(what, x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'{what}: rows of at least one value, got {tuple(x.shape)}')
     code = capi.dtype_code(what, 'x', x)
+    if x.numel() // x.shape[-1] * -(-x.shape[-1] // GROUP) > MAX_GROUPS:
+        raise ValueError(f'{what}: up to {MAX_GROUPS} groups of {GROUP} values, got {tuple(x.shape)}')
     capi.on_gpu(what, x)
     return x.contiguous(), code
 
@@ -135,9 +138,11 @@ def linear8_bwd_weight(dy, kept, bias=True):
     capi.on_gpu(what, dy)
     dy = dy.contiguous()
     m = dy.numel() // n
+    nbytes = lib.edgehip_linear8_workspace_bytes(code, m, n, k)
+    if nbytes == 0:
+        raise ValueError(f'{what}: a gradient of {n} x {k} is too large')
     dw = torch.empty((n, k), dtype=torch.float32, device=dy.device)
     db = torch.empty(n, dtype=torch.float32, device=dy.device) if bias else None
-    nbytes = lib.edgehip_linear8_workspace_bytes(code, m, n, k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
     with capi.on_device_of(dy) as stream:
         capi.check(lib.edgehip_linear8_bwd_weight(code, dy.data_ptr(), kept.codes.data_ptr(), kept.exps.data_ptr(), m, n, k,

@@ -44,8 +44,8 @@ def _describe(what, logits, taken, seq_ptr, mask):
         raise ValueError(f'{what}: logits must be [rows, classes], got {tuple(logits.shape)}')
     code = capi.dtype_code(what, 'logits', logits)
     rows, classes = logits.shape
-    if max(classes, 0 if seq_ptr is None else seq_ptr.numel() - 1) > 1 << 30:
-        raise ValueError(f'{what}: up to 2^30 classes and sequences')
+    if classes > 1 << 30 or seq_ptr is not None and seq_ptr.numel() > 1 << 24:
+        raise ValueError(f'{what}: up to 2^30 classes and 2^24 - 1 sequences')
     dev = logits.device
     if classes > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < classes:
         logits = logits.contiguous()

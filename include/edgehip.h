@@ -527,7 +527,7 @@ int edgehip_gate_norm_bwd(const edgehip_gate_norm* G, const void* dh_out, const 
  * [-120, 121] with max|x| <= 127 2^e (121 if there is none), and the whole numbers round-to-even(x 2^-e), held to
  * [-127, 127]; it stands for code * 2^e.  codes [M,K] int8,
  * exps [M, ceil(K/64)] int8.  e = -128: the group held an infinity or NaN, all of it stands for NaN.
- * pack8 / unpack8: x of `dtype`.  act8_fwd: y = act(x) and the checkpoint of x in one pass; act8_bwd:
+ * At most 2^29 - 32 groups in all.  pack8 / unpack8: x of `dtype`.  act8_fwd: y = act(x) and the checkpoint of x in one pass; act8_bwd:
  * dx = dy act'(kept x).  kind: 1 SiLU, 2 Mish (those of edgehip_act_fwd). */
 #define EDGEHIP_ACT_SILU 1
 #define EDGEHIP_ACT_MISH 2
@@ -548,7 +548,8 @@ int edgehip_linear8_bwd_weight(int32_t dtype, const void* dY, const int8_t* code
  * Row r of `logits` [rows, classes] (row_stride values from one row to the next) chose class taken[r]; sequence s is the
  * rows seq_ptr[s] .. seq_ptr[s+1]-1 (ascending from 0; the `aptr` of the active pairs is one).  A row counts if
  * mask[r] != 0 (mask NULL: every row), 0 <= taken[r] < classes and it lies in a sequence; the others have log-probability
- * 0 and gradient 0 whatever their logits hold.  dlogits is dense [rows, classes], of the logits' dtype, written whole. */
+ * 0 and gradient 0 whatever their logits hold.  dlogits is dense [rows, classes], of the logits' dtype, written whole.
+ * Up to 2^31 - 1 rows (fewer where a row takes several threads: 2^30 of 50 classes, 2^22 of 10^5) and 2^24 - 1 sequences. */
 #define EDGEHIP_TAKEN_I64 0
 #define EDGEHIP_TAKEN_U8 1               /* what edgehip_edge_resample puts out */
 typedef struct edgehip_logit_rows {

@@ -47,3 +47,61 @@ def test_types_of_choices():
         Q.taken_type = bad
         assert capi.lib.edgehip_tune_workspace_bytes(ctypes.byref(Q)) == 0
         assert capi.lib.edgehip_row_logp(ctypes.byref(Q), ctypes.c_void_p(4096), None) == capi.ERR_ARG
+
+
+def test_sizes_past_a_launch():
+    """A launch is a 32-bit number of threads along an axis: more are refused as too large, never handed to the runtime (which
+    would report a failed launch).  Nothing of that size is allocated here."""
+    import ctypes
+    import edgehip
+    from edgehip import capi, ckpt8
+    L, p, big = capi.lib, ctypes.c_void_p(4096), 1 << 60
+    byref = ctypes.byref
+    for m, k in ((1 << 29, 1), (1 << 29, 64), (1 << 28, 65), (1, 1 << 31)):
+        assert L.edgehip_pack8(1, p, m, k, p, p, None) == capi.ERR_TOO_LARGE
+        assert L.edgehip_unpack8(1, p, p, m, k, p, None) == capi.ERR_TOO_LARGE
+        assert L.edgehip_act8_fwd(1, 1, p, m, k, p, p, p, None) == capi.ERR_TOO_LARGE
+        assert L.edgehip_act8_bwd(1, 1, p, p, p, m, k, p, None) == capi.ERR_TOO_LARGE
+    assert L.edgehip_linear8_workspace_bytes(1, 64, 1 << 22, 1 << 22) == 0
+    assert L.edgehip_linear8_bwd_weight(1, p, p, p, 64, 1 << 22, 1 << 22, p, p, p, big, None) == capi.ERR_TOO_LARGE
+    wide = vec(1, 1).expand(1 << 29, 1)
+    for f in (edgehip.pack8, edgehip.act8):
+        with pytest.raises(ValueError, match='groups of 64'):
+            f(wide)
+    with pytest.raises(ValueError, match='too large'):
+        ckpt8.linear8_bwd_weight(_Gpu(vec(1, 1).expand(1, 1 << 22)), _kept(1 << 22))
+    # rows x threads of a row, and a block a sequence
+    O, R = capi.Policy(old_logp=4096, advantage=4096), capi.Preference(beta=0.1)
+
+    def codes(rows, classes, dtype, seqs=2):
+        Q = byref(capi.LogitRows(rows=rows, row_stride=classes, classes=classes, dtype=dtype, num_seqs=seqs, logits=4096, taken=4096, seq_ptr=4096))
+        return dict(logp=L.edgehip_row_logp(Q, p, None), fwd=L.edgehip_policy_loss_fwd(Q, byref(O), p, p, p, p, p, big, None),
+                    bwd=L.edgehip_policy_loss_bwd(Q, byref(O), p, p, big, None), grad=L.edgehip_policy_loss_grad(Q, byref(O), p, p, p, p, p, p, big, None),
+                    pfwd=L.edgehip_preference_loss_fwd(Q, byref(R), p, p, p, big, None), pbwd=L.edgehip_preference_loss_bwd(Q, byref(R), p, p, big, None),
+                    pgrad=L.edgehip_preference_loss_grad(Q, byref(R), p, p, p, p, big, None))
+    for rows, classes, dtype in ((1 << 30, 70, 0), (1 << 30, 70, 1), (1 << 28, 1025, 2), (1 << 22, 131073, 1), ((1 << 31) - 1, 1 << 20, 0)):
+        assert set(codes(rows, classes, dtype).values()) == {capi.ERR_TOO_LARGE}, (rows, classes, dtype)
+    assert set(codes(100, 4, 0, 1 << 24).values()) == {capi.ERR_TOO_LARGE}
+    with pytest.raises(ValueError, match='2\\^24 - 1 sequences'):
+        edgehip.preference_loss(vec(4, 3), torch.zeros(4, dtype=torch.int64), torch.zeros(1, dtype=torch.int64).expand((1 << 24) + 1))
+    with pytest.raises(ValueError, match='fixed capacity'):      # (too large an argument is a ValueError wherever C finds it)
+        capi.check(capi.ERR_TOO_LARGE, 'x')
+
+
+class _Gpu:
+    """A CPU tensor that says it is on a GPU: for checks that come behind that one."""
+    is_cuda = True
+
+    def __init__(self, t):
+        self.t = t
+
+    def contiguous(self):
+        return self
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def _kept(k):
+    from edgehip import ckpt8
+    return ckpt8.Packed8(vec(1, k, t=torch.int8), vec(1, -(-k // 64), t=torch.int8), torch.float32)
