@@ -24,7 +24,12 @@ class Packed8:
     __slots__ = ('codes', 'exps', 'dtype')
 
     def __init__(self, codes, exps, dtype):
-        self.codes, self.exps, self.dtype = codes, exps, dtype
+        if codes.dim() < 1 or codes.shape[-1] < 1 or codes.dtype != torch.int8 or exps.dtype != torch.int8:
+            raise ValueError(f'Packed8: int8 codes [..., K] and exps, got {tuple(codes.shape)} {codes.dtype}, {exps.dtype}')
+        rows, k = _rows(codes)
+        if exps.shape != (rows, -(-k // GROUP)) or exps.device != codes.device:
+            raise ValueError(f'Packed8: exps must be [{rows}, {-(-k // GROUP)}] beside codes {tuple(codes.shape)}, got {tuple(exps.shape)}')
+        self.codes, self.exps, self.dtype = codes.contiguous(), exps.contiguous(), dtype
 
     @property
     def shape(self):

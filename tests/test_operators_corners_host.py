@@ -105,3 +105,19 @@ class _Gpu:
 def _kept(k):
     from edgehip import ckpt8
     return ckpt8.Packed8(vec(1, k, t=torch.int8), vec(1, -(-k // 64), t=torch.int8), torch.float32)
+
+
+def test_a_checkpoint_put_together_by_hand():
+    """What the kernels read of a Packed8 is fixed when it is made: shapes and types that do not fit are refused (its exponents
+    would be read past their end), a strided part is made dense."""
+    from edgehip import ckpt8
+    i8 = lambda *s: vec(*s, t=torch.int8)
+    for codes, exps in ((i8(4, 130), i8(4, 2)), (i8(4, 130), i8(3, 3)), (i8(4, 130), i8(12)), (i8(4, 130), vec(4, 3, t=torch.uint8)),
+                        (vec(4, 130), i8(4, 3)), (i8(4, 0), i8(4, 0)), (torch.zeros((), dtype=torch.int8), i8(1, 1))):
+        with pytest.raises(ValueError, match='Packed8'):
+            ckpt8.Packed8(codes, exps, torch.float32)
+    for codes, exps in ((i8(4, 130), i8(4, 3)), (i8(130), i8(1, 3)), (i8(2, 3, 64), i8(6, 1)), (i8(0, 70), i8(0, 2))):
+        ckpt8.Packed8(codes, exps, torch.float32)
+    whole = torch.arange(8 * 128).to(torch.int8).view(8, 128)
+    part = ckpt8.Packed8(whole[::2, :64], i8(8, 2)[::2, :1], torch.float32)
+    assert part.codes.is_contiguous() and part.exps.is_contiguous() and torch.equal(part.codes, whole[::2, :64])
