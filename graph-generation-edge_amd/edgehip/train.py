@@ -282,10 +282,6 @@ class _Dropout(Function):
         return dx, None, None, None
 
 
-def linear(x, m):
-    return _Linear.apply(x, m.weight, m.bias)
-
-
 def act(x, kind=SILU):
     return _Act.apply(x, kind)
 
