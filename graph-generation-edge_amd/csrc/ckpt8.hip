@@ -2,9 +2,10 @@
 //
 // A row of K values is cut into groups of 64 (the last may be shorter).  A group shares a step 2^e, e the smallest
 // integer of [-120, 121] with max|x| <= 127 2^e, and keeps round-to-nearest-even(x 2^-e), a whole number of [-127, 127]:
-// off by at most 2^(e-1) <= max|x| / 127.  (Above 127 2^121 there is no such e: 121, and the codes end at 127 - a larger
-// step would stand for infinity at the top.)  A POWER OF TWO as the step makes a kept value code * 2^e exact in bf16 (7 significant
-// bits; bf16 has fp32's range), so in the weight gradient
+// off by at most 2^(e-1), which is at most max|x| / 127 but for a group at the smallest step, off by up to 2^-121 however
+// small its values are.  (Above 127 2^121 there is no such e: 121, and the codes end at 127 - a larger step would stand for
+// infinity at the top.)  A POWER OF TWO as the step makes a kept value code * 2^e exact in bf16 (7 significant bits; bf16 has
+// fp32's range), so in the weight gradient
 //     dW[n][k] = sum over m of dY[m][n] X8[m][k]
 // X8 enters the matrix instructions as ONE bf16 operand without error, and dY as 1 (bf16), 2 (fp16) or 3 (fp32) bf16
 // terms that add up to it exactly: every product is exact, sums are fp32.  An fp32 product needs 3 matrix

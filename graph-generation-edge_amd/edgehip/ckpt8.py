@@ -1,8 +1,8 @@
 """ckpt8.py - activations kept for the backward pass in 8 bits (csrc/ckpt8.hip).
 
 A row is cut into groups of 64 values; a group keeps whole numbers of [-127, 127] and the power of two they are multiples
-of: 1 + 1/64 bytes a value, off by at most 1/127 of the largest value of the group (half that at best).  `act8` and
-`linear8` are torch's activation and linear layer with such a checkpoint in place of their input; their forward results
+of: 1 + 1/64 bytes a value, off by at most 1/127 of the largest value of the group (half that at best; by up to 2^-121 in
+groups of values below 2^-113, whose step ends there, and values above 127 2^121 are held to that).  `act8` and `linear8` are torch's activation and linear layer with such a checkpoint in place of their input; their forward results
 are those of the exact input, only the gradients (of the activation's input, of the weight) read the kept values."""
 import torch
 from torch.autograd import Function
