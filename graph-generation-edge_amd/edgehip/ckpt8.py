@@ -2,8 +2,9 @@
 
 A row is cut into groups of 64 values; a group keeps whole numbers of [-127, 127] and the power of two they are multiples
 of: 1 + 1/64 bytes a value, off by at most 1/127 of the largest value of the group (half that at best; by up to 2^-121 in
-groups of values below 2^-113, whose step ends there, and values above 127 2^121 are held to that).  `act8` and `linear8` are torch's activation and linear layer with such a checkpoint in place of their input; their forward results
-are those of the exact input, only the gradients (of the activation's input, of the weight) read the kept values."""
+groups of values below 2^-113, whose step ends there, and values above 127 2^121 are held to that).  `act8` and `linear8`
+are torch's activation and linear layer with such a checkpoint in place of their input; their forward results are those of
+the exact input, only the gradients (of the activation's input, of the weight) read the kept values."""
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -56,11 +57,11 @@ def _rows(x):
     return (x.numel() // x.shape[-1], x.shape[-1]) if x.shape[-1] else (0, 0)
 
 
-def _input(what, x):
+def _input(what, x, kept=True):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'{what}: rows of at least one value, got {tuple(x.shape)}')
     code = capi.dtype_code(what, 'x', x)
-    if x.numel() // x.shape[-1] * -(-x.shape[-1] // GROUP) > MAX_GROUPS:
+    if kept and x.numel() // x.shape[-1] * -(-x.shape[-1] // GROUP) > MAX_GROUPS:
         raise ValueError(f'{what}: up to {MAX_GROUPS} groups of {GROUP} values, got {tuple(x.shape)}')
     capi.on_gpu(what, x)
     return x.contiguous(), code
@@ -193,7 +194,7 @@ def _aligned(t):
 class _Linear8(Function):
     @staticmethod
     def forward(ctx, x, w, b, kept):
-        x, _ = _input('linear8', x)
+        x, _ = _input('linear8', x, kept is not None)
         ctx.own = _own_products(x, w)
         if ctx.own:
             y = torch.empty((x.shape[0], w.shape[0]), dtype=x.dtype, device=x.device)

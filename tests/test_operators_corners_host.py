@@ -121,3 +121,12 @@ def test_a_checkpoint_put_together_by_hand():
     whole = torch.arange(8 * 128).to(torch.int8).view(8, 128)
     part = ckpt8.Packed8(whole[::2, :64], i8(8, 2)[::2, :1], torch.float32)
     assert part.codes.is_contiguous() and part.exps.is_contiguous() and torch.equal(part.codes, whole[::2, :64])
+
+
+def test_a_layer_that_keeps_nothing_takes_any_number_of_rows():
+    import edgehip
+    x, w = vec(1, 1).expand(1 << 29, 1), vec(3, 1)
+    with pytest.raises(ValueError, match='on a GPU'):
+        edgehip.linear8(x, w)
+    with pytest.raises(ValueError, match='groups of 64'):
+        edgehip.linear8(x, w.requires_grad_(True))
