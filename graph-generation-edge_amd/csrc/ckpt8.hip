@@ -560,7 +560,7 @@ __device__ static inline void dw_sum(const float* __restrict__ src, int64_t len,
     const int left = at < len ? (len - at < 4 ? (int)(len - at) : 4) : 0;
     if (len >= 4) {                                              // the last four columns are read whole and moved down
         const int64_t from = at + 4 <= len ? at : len - 4;
-#pragma unroll 8
+#pragma unroll 4
         for (int z = strip; z < np; z += STRIPS) {
             const eh_f32x4u v = *reinterpret_cast<const eh_f32x4u*>(src + z * len + from);
 #pragma unroll
