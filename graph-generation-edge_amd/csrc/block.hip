@@ -269,7 +269,9 @@ template <int DH, int DZ> struct gn_grad {
     float4 st;
 };
 
-// waves a SIMD: four (128 registers) with a 16-bit stream, three with fp32 (blocks of 1024 threads: four)
+// Waves a SIMD the registers are cut to: four (128 registers) with a 16-bit stream, three with fp32 (blocks of 1024 threads: four).
+// At four, up to 64 threads a row, the mean-and-variance kind spills 50-53 registers, the other kind 5-7; a row of whole waves spills
+// none, and with an fp32 stream takes 105-128, so that four waves fit there too.
 #define GN_BWD_WAVES(DH) ((DH) == EDGEHIP_F32 ? 3 : 4)
 template <int DH, int DZ, bool LAYER, int TPR, bool TINY = false>
 __global__ __launch_bounds__(GN_THREADS(TPR), (TPR == GN_ROW ? 4 : GN_BWD_WAVES(DH))) void k_gn_bwd(gn_args A) {
@@ -495,8 +497,9 @@ static int gn_tpr(int D) {
 }
 static size_t gn_par_bytes(int D, bool layer) { return (size_t)(D <= 512 ? gn_tpr(D) : (D + 511) / 512 * 64) * 8 * sizeof(float) * (layer ? 3 : 2); }
 static int gn_threads(int D) { return D <= 512 ? 256 : (D + 511) / 512 * 64; }
-// Rows a block owns.  Backward: as many blocks as the chip holds at once; more of them only add partials (5 D floats a block
-// at most) and a second, partly filled round.  Forward, no partials: two rounds of blocks, four where a block is one row
+// Rows a block owns.  Backward: no more blocks than GN_BWD_WAVES waves a SIMD make, whole blocks a CU; more of them add partials
+// (5 D floats a block at most) and a second, partly filled round.  (With an fp32 stream and rows of whole waves a fourth wave a
+// SIMD would fit; 7 or 8 waves a block, of 12 that are counted on, are one block a CU.)  Forward, no partials: two rounds of blocks, four where a block is one row
 // (16384 x 4096 bf16: 1024 blocks 110 us, 2048 96 us), but four rows a block where there are enough of them, as a block
 // reads the parameters once (5003 x 1101: one row a block 38 us, four 33 us).
 static int gn_rows_per_block(int64_t rows, int D, int stream_dtype, int bwd) {

@@ -238,9 +238,12 @@ extern "C" int edgehip_act8_bwd(int32_t dtype, int32_t kind, const void* dy, con
 // else is placed between its matrix instructions: two LDS images, and while a chunk of BM rows is multiplied, the next
 // one's registers (requested a chunk earlier) are turned and written and the one after is requested, in one run of
 // instructions without a branch; one barrier a chunk, which waits for LDS only, so that the requests stay in flight
-// across it.  16384 x 4096 x 4096 bf16: 526 us, 1046 TFLOP/s - the library's bf16 product of that shape, which has no codes
-// to turn, 527 us; the matrix pipe is busy 45 % of the cycles, vector instructions issue in 34 % (at 2.05 GHz).  fp16 /
-// fp32: 573 / 396 TFLOP/s (two / three terms).  78208 x 512 x 128 fp32: 54-60 us, 2.9 TB/s, T = 128 with two blocks a CU.
+// across it.  Launches back to back, the sums of partials with them: 16384 x 4096 x 4096 bf16 519-529 us, 1040-1060 TFLOP/s - the
+// library's bf16 product of that shape, which has no codes to turn, 520-527 us; the matrix pipe is busy 45 % of the cycles, vector
+// instructions issue in 34 %.  fp16 / fp32: 570 / 399 TFLOP/s (two / three terms).  78208 x 512 x 128 fp32, T = 128 with two
+// blocks a CU: 58 us, 2.9 TB/s of dY and codes; matrix pipe 23 %, vector instructions 36 % of the cycles, waves wait 36 % of
+// their time for their turn to issue and 23 % for memory or a barrier.  (One launch at a time, as a tracer runs them, the first is
+// 550-590 us, the second 61-63 us and 9 us.)
 // Not kept: a fixed pattern of one matrix instruction and 5 or 6 others (630-670 us); pieces of four rows with wider
 // reads and the exponents group by group (617 us).
 //

@@ -25,8 +25,9 @@
 // 8-value pieces of its row a thread keeps (64 registers)
 #define TN_KEEP(DT) ((DT) == EDGEHIP_F32 ? 8 : 16)
 // Classes up to which a thread takes a row alone.  Rows that are read once and kept: 128 bytes (10^6 x 33 / 10^6 x 48 bf16,
-// policy loss and gradient: four threads a row 105 / 102 us, one 62 / 70 us; 10^6 x 48 fp32: 128 us, 147 us).  Only written
-// (preference loss and gradient, 10^6 x 24 / 10^6 x 32 bf16: one 71 / 100 us, four 60 / 64 us): 16 classes.
+// policy loss and gradient: four threads a row 111 / 109 us, one 65 / 72 us; 10^6 x 48 fp32: 142 us either way, preference
+// loss and gradient 135, 144 us).  Only written (preference loss and gradient, 10^6 x 24 / 10^6 x 32 bf16: one 70 / 99 us, four
+// 59 / 66 us): 16 classes.
 #define TN_ALONE(DT, MODE) ((MODE) == 1 ? 16 : (DT) != EDGEHIP_F32 ? 64 : 32)
 
 struct tn_rows {
@@ -460,7 +461,7 @@ struct tn_final {
 };
 // Few rows: a sequence's block of 1024 threads adds them up itself (16 rows a thread at most), a launch less, two where the
 // count comes first.  More rows, which may all lie in one sequence, or more sequences than blocks that run at once go through
-// tn_sum's partials.  150 x 1000 fp32, preference loss and gradient: 24 us, 21 us; 8192 x 32003 bf16, policy: 232, 227 us.
+// tn_sum's partials.  150 x 1000 fp32, preference loss and gradient: 24 us, 21 us; 8192 x 32003 bf16, policy: 242, 238 us.
 static bool tn_direct(const tn_rows& T) { return T.R <= 16384 && T.S <= 512; }
 // totals of sequence g in every thread of the block, from the partials or from the rows (WHAT as in k_tn_part)
 template <int WHAT, bool DIRECT>
@@ -582,14 +583,13 @@ static void tn_go(const tn_rows& T, int tpr, dim3 grid, dim3 block, hipStream_t 
 template <int MODE> static int tn_alone(int dtype) { return dtype == EDGEHIP_F32 ? TN_ALONE(EDGEHIP_F32, MODE) : TN_ALONE(EDGEHIP_BF16, MODE); }
 template <int MODE>
 static int tn_threads(int dtype, int C) {
-    // Threads of a row: one for few classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 247 us, one
-    // 36 us), else as few as can keep it whole: what is done once per row is done by all of them, and a CU has rows in
-    // different phases (8192 x 32003 bf16: 1024 threads a row 382 us, 256 237 us; 10^5 x 513 bf16: 64 threads 213 us, 8
-    // 72 us).
+    // Threads of a row: one for few classes (10^6 x 9 bf16, policy loss and gradient: eight threads a row 143 us, one
+    // 40 us), else as few as can keep it whole: what is done once per row is done by all of them, and a CU has rows in
+    // different phases (8192 x 32003 bf16: 1024 threads a row 369 us, 256 238 us).
     const int per = 8 * (dtype == EDGEHIP_F32 ? TN_KEEP(EDGEHIP_F32) : TN_KEEP(EDGEHIP_BF16));
     if (C <= tn_alone<MODE>(dtype)) return 1;
     // (only written: wider runs pay more where a row has more than 128 bytes; preference over 10^6 x 48 fp32: four threads
-    // 154 us, eight 135 us; over 10^6 x 33 bf16: 97 us, 107 us)
+    // 156 us, eight 135 us; over 10^6 x 33 bf16: 77 us, 87 us)
     int tpr = MODE == 1 && C > (dtype == EDGEHIP_F32 ? 32 : 64) ? 8 : 4;
     while (tpr < 64 && C > tpr * per) tpr *= 2;
     if (C > 64 * per) tpr = 256;

@@ -585,7 +585,7 @@ typedef struct edgehip_preference {
     int32_t kind, mean;
 } edgehip_preference;
 /* ws: edgehip_tune_workspace_bytes(Q) bytes, 16-byte aligned.  *_fwd leaves in it what *_bwd (same arguments, weight: the
- * gradients of the losses) needs.  *_grad makes loss and gradient in one call (the policy loss in one pass over the logits; a
+ * gradients of the losses) needs; *_bwd writes scales to it, so that two on one ws go one after the other.  *_grad makes loss and gradient in one call (the policy loss in one pass over the logits; a
  * preference's gradient needs the sums of all rows first: two).  logp: [rows] or NULL. */
 size_t edgehip_tune_workspace_bytes(const edgehip_logit_rows* Q);
 int edgehip_policy_loss_fwd(const edgehip_logit_rows* Q, const edgehip_policy* O, float* loss, float* kl, int32_t* clipped,

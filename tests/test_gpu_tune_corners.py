@@ -168,3 +168,17 @@ def test_the_samplers_own_decisions():
     coef = -(adv.double() / n / b.num_graphs)[own][:, None]
     p = torch.softmax(logits.double(), 1)
     assert bool(((r.dlogits.double() - coef * (hot - p)).abs() <= 32 * U * coef.abs() * (hot + p) + 1e-30).all())
+
+
+def test_no_operator_loses_a_tangent():
+    """Forward mode: refused by every differentiable form."""
+    import edgehip
+    from torch.autograd import forward_ad
+    x, w, ptr = torch.randn(8, 64, device='cuda'), torch.randn(64, 64, device='cuda'), torch.tensor([0, 3, 8], device='cuda')
+    taken, old, adv = torch.zeros(8, dtype=torch.int64, device='cuda'), torch.zeros(8, device='cuda'), torch.ones(2, device='cuda')
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: edgehip.gate_norm(d, x), lambda: edgehip.gate_norm(x, d), lambda: edgehip.act8(d), lambda: edgehip.linear8(d, w),
+                  lambda: edgehip.policy_loss(d, taken, old, adv, ptr), lambda: edgehip.preference_loss(d, taken, ptr)):
+            with pytest.raises(NotImplementedError):
+                f()
