@@ -7,7 +7,7 @@ with root-mean-square or mean-and-variance norms.  `gate_norm` is the differenti
 import ctypes as C
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import capi
@@ -188,7 +188,8 @@ def gate_norm(h, z, *, w_pre=None, b_pre=None, w_post=None, b_post=None, gate=No
     """(h', y) of `gate_norm_fwd`, differentiable in h, z, the norms' parameters and the gate."""
     opts = dict(kind=kind, pre=pre, post=post, res_scale=res_scale, eps=eps)
     inputs = (h, z, w_pre, b_pre, w_post, b_post, gate)
-    capi.no_tangents('gate_norm', *inputs)
+    if forward_ad._current_level >= 0:
+        capi.no_tangents('gate_norm', *inputs)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
         return _GateNorm.apply(*inputs, row_ptr, opts)
     return gate_norm_fwd(h, z, w_pre=w_pre, b_pre=b_pre, w_post=w_post, b_post=b_post, gate=gate, row_ptr=row_ptr, **opts)[:2]

@@ -283,10 +283,9 @@ def on_gpu(what, t):
 
 
 def no_tangents(what, *tensors):
-    """Forward-mode derivatives: there are none, and a tensor's tangent must not get lost on the way past autograd."""
+    """Forward-mode derivatives: there are none, and a tensor's tangent must not get lost on the way past autograd.  (Asked where
+    forward_ad has a level open.)"""
     from torch.autograd import forward_ad
-    if forward_ad._current_level < 0:
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f'{what}: no forward-mode derivative (gradients are made by its backward pass)')

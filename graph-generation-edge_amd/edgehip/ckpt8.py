@@ -6,7 +6,7 @@ groups of values below 2^-113, whose step ends there, and values above 127 2^121
 are torch's activation and linear layer with such a checkpoint in place of their input; their forward results are those of
 the exact input, only the gradients (of the activation's input, of the weight) read the kept values."""
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import capi
@@ -31,6 +31,13 @@ class Packed8:
         if exps.shape != (rows, -(-k // GROUP)) or exps.device != codes.device:
             raise ValueError(f'Packed8: exps must be [{rows}, {-(-k // GROUP)}] beside codes {tuple(codes.shape)}, got {tuple(exps.shape)}')
         self.codes, self.exps, self.dtype = codes.contiguous(), exps.contiguous(), dtype
+
+    @classmethod
+    def _of(cls, codes, exps, dtype):
+        """Of tensors that fit each other by their making."""
+        self = cls.__new__(cls)
+        self.codes, self.exps, self.dtype = codes, exps, dtype
+        return self
 
     @property
     def shape(self):
@@ -61,7 +68,7 @@ def _input(what, x, kept=True):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'{what}: rows of at least one value, got {tuple(x.shape)}')
     code = capi.dtype_code(what, 'x', x)
-    if kept and x.numel() // x.shape[-1] * -(-x.shape[-1] // GROUP) > MAX_GROUPS:
+    if kept and x.numel() > MAX_GROUPS and x.numel() // x.shape[-1] * -(-x.shape[-1] // GROUP) > MAX_GROUPS:
         raise ValueError(f'{what}: up to {MAX_GROUPS} groups of {GROUP} values, got {tuple(x.shape)}')
     capi.on_gpu(what, x)
     return x.contiguous(), code
@@ -75,8 +82,8 @@ def _kind(what, kind):
 
 def _new(x):
     rows, k = _rows(x)
-    return Packed8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-                   torch.empty((rows, -(-k // GROUP)), dtype=torch.int8, device=x.device), x.dtype)
+    return Packed8._of(torch.empty(x.shape, dtype=torch.int8, device=x.device),
+                       torch.empty((rows, -(-k // GROUP)), dtype=torch.int8, device=x.device), x.dtype)
 
 
 def pack8(x):
@@ -168,12 +175,13 @@ class _Act8(Function):
     @once_differentiable
     def backward(ctx, dy):
         dtype, kind = ctx.kept
-        return act8_bwd(dy, Packed8(*ctx.saved_tensors, dtype), kind), None
+        return act8_bwd(dy, Packed8._of(*ctx.saved_tensors, dtype), kind), None
 
 
 def act8(x, kind='silu'):
     """act(x), keeping x in 8 bits for the backward pass."""
-    capi.no_tangents('act8', x)
+    if forward_ad._current_level >= 0:
+        capi.no_tangents('act8', x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Act8.apply(x, kind)
     return act8_fwd(x, kind)[0]
@@ -231,13 +239,13 @@ class _Linear8(Function):
                     dx = torch.matmul(dy, w)
         want_db = ctx.has_bias and ctx.needs_input_grad[2]
         if ctx.needs_input_grad[1]:
-            dw, db = linear8_bwd_weight(dy, Packed8(codes, exps, ctx.dtype), bias=want_db)
+            dw, db = linear8_bwd_weight(dy, Packed8._of(codes, exps, ctx.dtype), bias=want_db)
             dw = dw.to(w.dtype)
             db = db.to(w.dtype) if want_db else None
         elif want_db:
             # (no library sum: a captured one can hold a memory-set node; the checkpoint of an input of one zero is a stand-in)
             none = torch.zeros(dy.shape[:-1] + (1,), dtype=torch.int8, device=dy.device)
-            db = linear8_bwd_weight(dy, Packed8(none, none.reshape(-1, 1), ctx.dtype))[1].to(w.dtype)
+            db = linear8_bwd_weight(dy, Packed8._of(none, none.reshape(-1, 1), ctx.dtype))[1].to(w.dtype)
         return dx, dw, db, None
 
 
