@@ -54,7 +54,8 @@ struct tn_rows {
 };
 
 __device__ static inline bool tn_counts(const tn_rows& T, int64_t r, int64_t& a) {
-    a = T.taken8 ? (int64_t)static_cast<const uint8_t*>(T.taken)[r] : static_cast<const int64_t*>(T.taken)[r];      // (all requests at once, no branch between them)
+    // (all requests at once, no branch between them)
+    a = T.taken8 ? (int64_t)static_cast<const uint8_t*>(T.taken)[r] : static_cast<const int64_t*>(T.taken)[r];
     bool on = (a >= 0) & (a < T.C);
     if (T.mask) on &= T.mask[r] != 0;
     if (T.seq_ptr) on &= (r >= T.seq_ptr[0]) & (r < T.seq_ptr[T.S]);
@@ -111,9 +112,9 @@ __device__ static inline float tn_kl(float d, float& slope) {
     return d > 80.0f ? e : slope - d;                            // (an infinite gap is not NaN)
 }
 
-// e^x, x <= 700 or NaN (below -150: e^-150), in fp64 to 3.5e-8 (rms 6e-9, mean below 2e-10).  e^x = 2^n (1 + q): n = rint(x log2 e), r = x - n ln 2, ln 2
-// as 16 bits (n times them is exact) and the rest; q = e^r - 1 = r + r^2 P(r) in fp32, where its rounding is at most 2^-26; P
-// has the smallest largest error over |r| <= ln 2 / 2, 5e-10.  A row of few classes has no many terms to average over and a
+// e^x, x <= 700 or NaN (below -150: e^-150), in fp64 to 3.5e-8 (rms 6e-9, mean below 2e-10).  e^x = 2^n (1 + q):
+// n = rint(x log2 e), r = x - n ln 2, ln 2 as 16 bits (n times them is exact) and the rest; q = e^r - 1 = r + r^2 P(r) in fp32,
+// where its rounding is at most 2^-26; P has the smallest largest error over |r| <= ln 2 / 2, 5e-10.  A row of few classes has no many terms to average over and a
 // preference's margin is the difference of sums over many such rows: rounded to fp32 and added up there, a row's
 // log-probability was off by 3e-8 to 7e-8, all margins by that times the root of their rows and more.
 __device__ static inline double tn_exp64(float x) {
@@ -207,9 +208,9 @@ __device__ static inline void tn_wave_part(double (&v)[WHAT == 1 ? 2 : 1], bool 
     }
 }
 
-// e^x in fp32 by the hardware's power of two, for the sums of rows of many classes and for every value of a gradient.  The fp32 constant log2(e) alone is 1.3e-8 off:
-// every term of a row would be off to the same side by that times |x|.  With the constant's second part the error of a term
-// is that of rounding x log2(e), to either side, and the instruction's own (mean -3e-9).
+// e^x in fp32 by the hardware's power of two, for the sums of rows of many classes and for every value of a gradient.  The fp32
+// constant log2(e) alone is 1.3e-8 off: every term of a row would be off to the same side by that times |x|.  With the
+// constant's second part the error of a term is that of rounding x log2(e), to either side, and the instruction's own (mean -3e-9).
 __device__ static inline float tn_exp(float x) {
     constexpr float HI = 1.44269502162933349609f, LO = 1.92596298909109e-8f;
     return __builtin_amdgcn_exp2f(__builtin_fmaf(x, HI, x * LO));
@@ -260,7 +261,7 @@ __device__ static inline void tn_row_merge(float& m, double& s, float* lds_m, do
     }
 }
 
-// n of eight more values (N: how many at most) into the running pair.  NaN: the sum becomes NaN and stays it.  FEW: each
+// n of eight more values into the running pair.  NaN: the sum becomes NaN and stays it.  FEW: each
 // exponential and the sum in fp64; else eight are added up in fp32, which many pieces average, and the pieces in fp64.
 template <bool FEW>
 __device__ static inline void tn_add8(float& m, double& s, const float (&v)[8], int n = 8) {
